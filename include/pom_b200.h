@@ -631,6 +631,95 @@ int pom_peer_allreduce_flat(const pom_peer_comm* c, unsigned long long n_floats,
  * flat_floats multiples of 8.  The fp32 accumulators are left as they were. */
 int pom_peer_allreduce_flat_bf16(const pom_peer_comm* c, unsigned long long n_floats, int* status, void* stream);
 
+/* ------------------------------------------------------------------------------------------
+ * Operators of a residual block around the mixer: layer norm, the linear map of a feed-forward block, rotary positions
+ * of several axes.  No counterpart in the reference, which leaves these to torch.nn.  Strides are in elements; the last
+ * dimension is contiguous.  The same call gives the same bits every time.
+ */
+
+/* Layer norm over the last dimension of (M, D) rows.  stats (M, 2) fp32 holds mean and 1 / sqrt(var + eps) per row: the
+ * forward call writes it where it is given, the backward call reads it.  weight and bias may be NULL (1 and 0; bias only
+ * with weight).  dtype is that of x, y, dy and dx; wdtype that of weight, bias, dweight and dbias (POM_F32, or POM_BF16
+ * with bf16 rows).  Backward: any of dx, dweight and dbias may be NULL; with a weight gradient, workspace of
+ * pom_layer_norm_bwd_workspace bytes (16-byte aligned). */
+typedef struct pom_layer_norm_args {
+  const void* x;
+  const void* weight;
+  const void* bias;
+  void* y;
+  float* stats;
+  const void* dy;
+  void* dx;
+  void* dweight;
+  void* dbias;
+  void* workspace;
+  int64_t M, ldx, ldy, ld_dy, ld_dx;
+  int32_t D;
+  int32_t dtype, wdtype;
+  float eps;
+} pom_layer_norm_args;
+int pom_layer_norm_fwd(const pom_layer_norm_args* a, void* stream);
+uint64_t pom_layer_norm_bwd_workspace(const pom_layer_norm_args* a);
+int pom_layer_norm_bwd(const pom_layer_norm_args* a, void* stream);
+
+enum { POM_ACT_NONE = 0, POM_ACT_GELU = 1, POM_ACT_GELU_TANH = 2, POM_ACT_SILU = 3, POM_ACT_RELU = 4 };
+
+/* y = act(x w^T + bias) + residual with x (M, K), w (N, K), bias (N), residual and y (M, N).
+ *
+ * Forward (pom_linear_fwd): slope, where given, receives act'(x w^T + bias) as contiguous (M, N) values of dtype: what
+ * the backward call needs of the forward pass.  bf16: K, N and every row stride multiples of 8, 16-byte aligned
+ * addresses.  float32: only calls for which pom_linear_few_rows is nonzero; for the others z = x w^T comes from
+ * pom_gemm_f32 or pom_gemm_f32_planes, and pom_linear_epilogue does the rest (y may be z).
+ *
+ * Backward (pom_linear_bwd): dz = dy * slope (slope NULL: dz = dy), dbias = column sums of dz, dw = dz^T x (N, K) and
+ * dx = dz w (M, K), both contiguous; any of the three may be NULL.  dz: NULL, or where to put it (contiguous).  float32:
+ * dz and dbias only (dx and dw NULL).  workspace: pom_linear_bwd_workspace bytes, 16-byte aligned. */
+typedef struct pom_linear_args {
+  const void* x;
+  const void* w;
+  const void* bias;
+  const void* residual;
+  void* y;
+  void* slope;
+  const void* dy;
+  void* dz;
+  void* dx;
+  void* dw;
+  void* dbias;
+  void* workspace;
+  int64_t M, N, K;
+  int64_t ldx, ldw, ldr, ldy, ld_dy;
+  int32_t act, dtype, bias_dtype, reserved0;
+} pom_linear_args;
+int pom_linear_few_rows(const pom_linear_args* a);
+int pom_linear_fwd(const pom_linear_args* a, int* status, void* stream);
+int pom_linear_epilogue(const pom_linear_args* a, const float* z, int64_t ldz, void* stream);
+uint64_t pom_linear_bwd_workspace(const pom_linear_args* a);
+int pom_linear_bwd(const pom_linear_args* a, int* status, void* stream);
+
+#define POM_ROPE_MAX_AXES 4
+
+/* Rotation of x (B, N, H, D) by the positions of `axes` axes: section a is 2 * pairs[a] channels wide (in the order of the
+ * axes), channel k of it is paired with k + pairs[a] and turned by cos / sin[pos_a][k] of the axis' (len, pairs) table;
+ * channels behind the sections are copied.  transpose turns the other way (the backward pass).  pos (N, axes), or
+ * (B, N, axes) with pos_per_sample.  x has strides xs_*, y is contiguous.  A position outside [0, len) makes its
+ * section NaN; nothing outside the tables is read. */
+typedef struct pom_rope_axes_args {
+  const void* x;
+  void* y;
+  const int64_t* pos;
+  const float* cos[POM_ROPE_MAX_AXES];
+  const float* sin[POM_ROPE_MAX_AXES];
+  int32_t len[POM_ROPE_MAX_AXES], pairs[POM_ROPE_MAX_AXES];
+  int64_t xs_b, xs_n, xs_h;
+  int64_t B, N;
+  int32_t H, D, axes, dtype;
+  int32_t pos_per_sample, transpose;
+} pom_rope_axes_args;
+int pom_rope_axes(const pom_rope_axes_args* a, void* stream);
+/* Smallest and largest value of every column of the (rows, axes) positions: info[2 a], info[2 a + 1]. */
+int pom_pos_range(const int64_t* pos, int64_t rows, int32_t axes, int64_t* info, void* stream);
+
 /* Asynchronous device-to-device copy of `bytes` bytes on the stream (cudaMemcpyAsync; no kernel). */
 int pom_copy_bytes(void* dst, const void* src, int64_t bytes, void* stream);
 

@@ -181,6 +181,46 @@ class LayerArgs(C.Structure):
     ]
 
 
+class LayerNormArgs(C.Structure):
+    _fields_ = [
+        ("x", C.c_void_p), ("weight", C.c_void_p), ("bias", C.c_void_p), ("y", C.c_void_p), ("stats", C.c_void_p),
+        ("dy", C.c_void_p), ("dx", C.c_void_p), ("dweight", C.c_void_p), ("dbias", C.c_void_p),
+        ("workspace", C.c_void_p),
+        ("M", C.c_int64), ("ldx", C.c_int64), ("ldy", C.c_int64), ("ld_dy", C.c_int64), ("ld_dx", C.c_int64),
+        ("D", C.c_int32), ("dtype", C.c_int32), ("wdtype", C.c_int32), ("eps", C.c_float),
+    ]
+
+
+ACTIVATIONS = {None: 0, "gelu": 1, "gelu_tanh": 2, "silu": 3, "relu": 4}
+
+
+class LinearArgs(C.Structure):
+    _fields_ = [
+        ("x", C.c_void_p), ("w", C.c_void_p), ("bias", C.c_void_p), ("residual", C.c_void_p), ("y", C.c_void_p),
+        ("slope", C.c_void_p),
+        ("dy", C.c_void_p), ("dz", C.c_void_p), ("dx", C.c_void_p), ("dw", C.c_void_p), ("dbias", C.c_void_p),
+        ("workspace", C.c_void_p),
+        ("M", C.c_int64), ("N", C.c_int64), ("K", C.c_int64),
+        ("ldx", C.c_int64), ("ldw", C.c_int64), ("ldr", C.c_int64), ("ldy", C.c_int64), ("ld_dy", C.c_int64),
+        ("act", C.c_int32), ("dtype", C.c_int32), ("bias_dtype", C.c_int32), ("reserved0", C.c_int32),
+    ]
+
+
+ROPE_MAX_AXES = 4
+
+
+class RopeAxesArgs(C.Structure):
+    _fields_ = [
+        ("x", C.c_void_p), ("y", C.c_void_p), ("pos", C.c_void_p),
+        ("cos", C.c_void_p * ROPE_MAX_AXES), ("sin", C.c_void_p * ROPE_MAX_AXES),
+        ("len", C.c_int32 * ROPE_MAX_AXES), ("pairs", C.c_int32 * ROPE_MAX_AXES),
+        ("xs_b", C.c_int64), ("xs_n", C.c_int64), ("xs_h", C.c_int64),
+        ("B", C.c_int64), ("N", C.c_int64),
+        ("H", C.c_int32), ("D", C.c_int32), ("axes", C.c_int32), ("dtype", C.c_int32),
+        ("pos_per_sample", C.c_int32), ("transpose", C.c_int32),
+    ]
+
+
 PEER_MAX_RANKS = 16
 PEER_HANDLE_BYTES = 64
 PEER_SUM_ALL, PEER_SUM_BEFORE, PEER_SUM_AFTER = 0, 1, 2
@@ -259,6 +299,16 @@ _SIGNATURES = {
     "pom_peer_exchange": (C.c_int, [C.POINTER(PeerComm), C.POINTER(PeerXchgArgs), C.c_void_p, C.c_void_p]),
     "pom_peer_allreduce_flat": (C.c_int, [C.POINTER(PeerComm), C.c_ulonglong, C.c_void_p, C.c_void_p]),
     "pom_peer_allreduce_flat_bf16": (C.c_int, [C.POINTER(PeerComm), C.c_ulonglong, C.c_void_p, C.c_void_p]),
+    "pom_layer_norm_fwd": (C.c_int, [C.POINTER(LayerNormArgs), C.c_void_p]),
+    "pom_layer_norm_bwd_workspace": (C.c_uint64, [C.POINTER(LayerNormArgs)]),
+    "pom_layer_norm_bwd": (C.c_int, [C.POINTER(LayerNormArgs), C.c_void_p]),
+    "pom_linear_few_rows": (C.c_int, [C.POINTER(LinearArgs)]),
+    "pom_linear_fwd": (C.c_int, [C.POINTER(LinearArgs), C.c_void_p, C.c_void_p]),
+    "pom_linear_epilogue": (C.c_int, [C.POINTER(LinearArgs), C.c_void_p, C.c_int64, C.c_void_p]),
+    "pom_linear_bwd_workspace": (C.c_uint64, [C.POINTER(LinearArgs)]),
+    "pom_linear_bwd": (C.c_int, [C.POINTER(LinearArgs), C.c_void_p, C.c_void_p]),
+    "pom_rope_axes": (C.c_int, [C.POINTER(RopeAxesArgs), C.c_void_p]),
+    "pom_pos_range": (C.c_int, [C.c_void_p, C.c_int64, C.c_int32, C.c_void_p, C.c_void_p]),
     "pom_copy_bytes": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int64, C.c_void_p]),
 }
 

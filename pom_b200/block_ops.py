@@ -1,0 +1,238 @@
+"""Operators of a residual block around the mixer, on the CUDA kernels of this package: layer norm, the linear map with
+bias, activation and residual, and rotary positions of several axes.
+
+The reference leaves these to ``torch.nn`` (its README builds the blocks around ``PoM`` from ``nn.LayerNorm`` and
+``nn.Linear``) and has rotary positions of one and two axes (pom/pom_rope.py:152-235).  All three take bfloat16 and
+float32 tensors, any strides (rows that do not follow one another in one step are copied), run on the tensors' device
+and current stream, are differentiable once, and may be captured into CUDA graphs.  They give the same bits on every
+run.  ``pom_b200.operators`` exports them.
+"""
+from __future__ import annotations
+
+from typing import Optional, Sequence, Tuple
+
+import torch
+import torch.nn.functional as F
+from torch.autograd.function import once_differentiable
+
+from . import _abi, ops
+from .functional import eager_only, on_tensor_device
+
+_any_autocast = getattr(torch._C, "_is_any_autocast_enabled", lambda: True)
+_TYPES = (torch.bfloat16, torch.float32)
+
+
+def _check_tokens(x: torch.Tensor, name: str = "x") -> None:
+    # where it lives is checked with the other tensors of the call (ops._require_cuda)
+    if not isinstance(x, torch.Tensor):
+        raise TypeError(f"{name} must be a tensor, got {type(x).__name__}")
+    if x.dtype not in _TYPES:
+        raise TypeError(f"unsupported dtype {x.dtype} of {name}; use bfloat16 or float32")
+
+
+def _tracked(*tensors) -> bool:
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+
+
+# --------------------------------------------------------------------------- layer norm
+class _LayerNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, eps):
+        y, stats = ops.layer_norm_fwd(x, weight, bias, eps, True)
+        ctx.save_for_backward(x, weight, stats)
+        return y
+
+    @staticmethod
+    @once_differentiable
+    @on_tensor_device
+    def backward(ctx, g):
+        x, weight, stats = ctx.saved_tensors
+        nx, nw, nb, _ = ctx.needs_input_grad
+        dx, dw, db = ops.layer_norm_bwd(g, x, weight, stats, want_dx=nx, want_dw=nw, want_db=nb)
+        return dx, dw, db, None
+
+
+@eager_only
+@on_tensor_device
+def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None,
+               eps: float = 1e-5) -> torch.Tensor:
+    """``(x - mean) / sqrt(var + eps) * weight + bias`` over the last dimension, in x's dtype.
+
+    x (..., D) bfloat16 or float32; ``weight`` and ``bias`` (D,) in x's dtype or float32 (``bias`` only with ``weight``).
+    Statistics and sums are float32.  A row with an infinity or a NaN comes out NaN."""
+    _check_tokens(x)
+    if x.dim() < 1 or x.shape[-1] == 0:
+        raise ValueError(f"expected a (..., D) tensor with D > 0, got {tuple(x.shape)}")
+    if weight is None:
+        if bias is not None:
+            raise ValueError("layer_norm takes a bias only together with a weight")
+    else:
+        D = x.shape[-1]
+        for t, name in ((weight, "weight"), (bias, "bias")):
+            if t is None:
+                continue
+            _check_tokens(t, name)
+            if t.dim() != 1 or t.shape[0] != D:
+                raise ValueError(f"{name} must have shape ({D},), got {tuple(t.shape)}")
+        if weight.dtype != torch.float32 and weight.dtype != x.dtype:
+            weight = weight.float()  # bf16 parameters beside float32 rows
+        if not weight.is_contiguous():
+            weight = weight.contiguous()
+        if bias is not None:
+            if bias.dtype != weight.dtype:
+                if weight.dtype == torch.bfloat16:
+                    weight = weight.float()
+                bias = bias.to(weight.dtype)
+            if not bias.is_contiguous():
+                bias = bias.contiguous()
+    if _tracked(x, weight, bias):
+        return _LayerNorm.apply(x, weight, bias, eps)
+    return ops.layer_norm_fwd(x, weight, bias, eps, False)[0]
+
+
+# --------------------------------------------------------------------------- linear map
+class _Linear(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, residual, act):
+        nx, nw, nb, _, _ = ctx.needs_input_grad
+        y, slope = ops.linear_fwd(x, weight, bias, act, residual, act is not None and (nx or nw or nb))
+        ctx.save_for_backward(x, weight, slope)
+        ctx.bias_dtype = bias.dtype if nb else None
+        return y
+
+    @staticmethod
+    @once_differentiable
+    @on_tensor_device
+    def backward(ctx, g):
+        x, weight, slope = ctx.saved_tensors
+        nx, nw, nb, nr, _ = ctx.needs_input_grad
+        dx = dw = db = None
+        if nx or nw or nb:
+            dx, dw, db = ops.linear_bwd(g, x, weight, slope, want_dx=nx, want_dw=nw, bias_dtype=ctx.bias_dtype)
+        return dx, dw, db, (g if nr else None), None
+
+
+def _pad8(n: int) -> int:
+    return -n % 8
+
+
+@eager_only
+@on_tensor_device
+def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None, *,
+           activation: Optional[str] = None, residual: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``activation(x · weightᵀ + bias) + residual`` in one product.
+
+    x (..., K) and ``weight`` (N, K) of one dtype, bfloat16 or float32; ``bias`` (N,) in that dtype or float32;
+    ``residual`` of the output's shape and dtype; ``activation`` None, "gelu" (exact), "gelu_tanh", "silu" or "relu".
+    Sums, bias, activation and residual are float32, rounded once.  With an activation and a gradient to come, its slope
+    is kept in x's dtype and the backward pass multiplies by it.  bfloat16 widths that are not multiples of 8 are padded
+    with zeros (a copy of the operands).  Under ``torch.autocast("cuda", torch.bfloat16)`` x, ``weight`` and ``residual``
+    are cast to bfloat16 on the way in."""
+    _check_tokens(x)
+    _check_tokens(weight, "weight")
+    if activation not in _abi.ACTIVATIONS:
+        raise ValueError(f"activation must be one of {sorted(k for k in _abi.ACTIVATIONS if k)} or None, got {activation!r}")
+    if weight.dim() != 2 or x.dim() < 1 or x.shape[-1] != weight.shape[1] or 0 in weight.shape:
+        raise ValueError(f"expected x (..., K) and weight (N, K) with N, K > 0, got {tuple(x.shape)} and {tuple(weight.shape)}")
+    N, K = weight.shape
+    if bias is not None:
+        _check_tokens(bias, "bias")
+        if bias.shape != (N,):
+            raise ValueError(f"bias must have shape ({N},), got {tuple(bias.shape)}")
+    if residual is not None:
+        _check_tokens(residual, "residual")
+        if residual.shape[:-1] != x.shape[:-1] or residual.shape[-1] != N:
+            raise ValueError(f"residual must have the output's shape {(*x.shape[:-1], N)}, got {tuple(residual.shape)}")
+    if _any_autocast():
+        from .pom import PoM  # the module decides what autocast means for its projections; the same here
+
+        dt = PoM._autocast_dtype()
+        if dt is not None:
+            x, weight = x.to(dt), weight.to(dt)
+            residual = None if residual is None else residual.to(dt)
+    if weight.dtype != x.dtype or (residual is not None and residual.dtype != x.dtype):
+        raise TypeError("x, weight and residual must share one dtype")
+    if bias is not None:
+        if x.dtype == torch.float32 and bias.dtype != torch.float32:
+            bias = bias.float()
+        bias = bias.contiguous()
+    if x.dtype == torch.bfloat16 and (K % 8 or N % 8):
+        kp, n_pad = _pad8(K), _pad8(N)
+        y = linear(F.pad(x, (0, kp)), F.pad(weight, (0, kp, 0, n_pad)), None if bias is None else F.pad(bias, (0, n_pad)),
+                   activation=activation, residual=None if residual is None else F.pad(residual, (0, n_pad)))
+        return y[..., :N].contiguous() if n_pad else y
+    if _tracked(x, weight, bias, residual):
+        return _Linear.apply(x, weight, bias, residual, activation)
+    return ops.linear_fwd(x, weight, bias, activation, residual, False)[0]
+
+
+# --------------------------------------------------------------------------- rotary positions of several axes
+class _RotateAxes(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, pos, tables):
+        ctx.pos, ctx.tables = pos, tables
+        return ops.rope_axes(x, pos, tables)
+
+    @staticmethod
+    @once_differentiable
+    @on_tensor_device
+    def backward(ctx, g):
+        return ops.rope_axes(g, ctx.pos, ctx.tables, transpose=True), None, None
+
+
+@eager_only
+@on_tensor_device
+def apply_rope_axes(x: torch.Tensor, positions: torch.Tensor, tables: Sequence[Tuple[torch.Tensor, torch.Tensor]], *,
+                    validate: bool = True) -> torch.Tensor:
+    """Rotary positions of one to four axes, e.g. (time, height, width) of video tokens.
+
+    x (B, N, D), or (B, N, H, D) with heads that share the angles.  ``tables``: per axis a (cos, sin) pair of
+    (rows, s_a) tensors (see :func:`precompute_freqs_axes`); the axes' sections of 2 s_a channels follow one another, and
+    inside a section channel k pairs with k + s_a, as :func:`apply_rope_2d` pairs its two halves; channels behind the
+    last section pass.  ``positions`` (N, A) for all samples, or (B, N, A).
+
+    ``validate``: an IndexError for a position outside its table, at the price of a synchronising read the first time a
+    position tensor is seen.  Without it nothing is read back, and such a position makes its section of the token NaN."""
+    _check_tokens(x)
+    if x.dim() not in (3, 4):
+        raise ValueError(f"expected a (B, N, D) or (B, N, H, D) tensor, got {tuple(x.shape)}")
+    if not 1 <= len(tables) <= _abi.ROPE_MAX_AXES:
+        raise ValueError(f"1 to {_abi.ROPE_MAX_AXES} axes, got {len(tables)}")
+    D, axes, width, tabs = x.shape[-1], len(tables), 0, []
+    for i, (cos, sin) in enumerate(tables):
+        if cos.dim() != 2 or cos.shape != sin.shape or 0 in cos.shape:
+            raise ValueError(f"tables[{i}] must be two (rows, pairs) tensors of one shape, got {tuple(cos.shape)} and "
+                             f"{tuple(sin.shape)}")
+        width += 2 * cos.shape[1]
+        tabs.append(tuple(t if t.dtype == torch.float32 and t.device == x.device and t.is_contiguous()
+                          else t.to(device=x.device, dtype=torch.float32).contiguous() for t in (cos, sin)))
+    if width > D:
+        raise ValueError(f"the axes rotate {width} channels but x has {D}")
+    B, N = x.shape[:2]
+    if tuple(positions.shape) not in ((N, axes), (B, N, axes)):
+        raise ValueError(f"positions must have shape ({N}, {axes}) or ({B}, {N}, {axes}), got {tuple(positions.shape)}")
+    if positions.dtype.is_floating_point or positions.dtype == torch.bool:
+        raise TypeError(f"positions must be integers, got {positions.dtype}")
+    if validate and positions.numel():
+        on_gpu = positions if positions.dtype == torch.int64 and positions.device == x.device else \
+            positions.to(device=x.device, dtype=torch.int64)
+        for a, ((lo, hi), (cos, _)) in enumerate(zip(ops.pos_range(on_gpu), tabs)):
+            if lo < 0 or hi >= cos.shape[0]:
+                raise IndexError(f"positions of axis {a} span [{lo}, {hi}] but its table has {cos.shape[0]} rows")
+        positions = on_gpu
+    pos = positions.to(device=x.device, dtype=torch.int64).contiguous()
+    if x.requires_grad and torch.is_grad_enabled():
+        return _RotateAxes.apply(x, pos, tabs)
+    return ops.rope_axes(x, pos, tabs)
+
+
+def precompute_freqs_axes(pairs: Sequence[int], rows: Sequence[int], base: float = 10000.0):
+    """One (cos, sin) pair of (rows[a], pairs[a]) float32 tables per axis, angle position * base^(-k / pairs[a]); formed in
+    64 bits, so that far positions keep their angles.  With equal axes the tables of
+    :func:`pom_b200.pom_rope.precompute_freqs_2d`."""
+    out = []
+    for s, n in zip(pairs, rows):
+        f = float(base) ** (-torch.arange(s, dtype=torch.float64) / s)
+        ang = torch.outer(torch.arange(n, dtype=torch.float64), f)
+        out.append((ang.cos().float(), ang.sin().float()))
+    return out

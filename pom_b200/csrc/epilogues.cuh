@@ -99,7 +99,8 @@ struct EpiStore {
     void* C;                 // fp32 modes only (bf16 output goes through maps.out0)
     long long ldc;           // elements
     long long batch_stride;  // elements between batches
-    int mode;                // 0: bf16 store, 1: fp32 store, 2: fp32 atomic add (split-K)
+    long long split_stride;  // fp32 store only: elements between the outputs of consecutive K splits
+    int mode;                // 0: bf16 store, 1: fp32 store (one output per K split), 2: fp32 atomic add (split-K)
     float alpha;
     int act;                 // bf16 store only: 0 none, 1 exact GELU 0.5 x (1 + erf(x / sqrt 2))
     const __nv_bfloat16* residual;  // bf16 store only: added after the activation (row stride ldr), or null
@@ -121,7 +122,8 @@ struct EpiStore {
                                              EpiIO& io, int) {
     const int row = quarter * 32 + lane;
     const bool row_ok = row < t.rows_valid;
-    const long long off = static_cast<long long>(t.b) * p.batch_stride + static_cast<long long>(t.row0 + row) * p.ldc;
+    const long long off = static_cast<long long>(t.b) * p.batch_stride + static_cast<long long>(t.row0 + row) * p.ldc +
+                          static_cast<long long>(t.split) * p.split_stride;
     int flip = 0;
 #pragma unroll 1
     for (int c = half; c < BN / 32; c += kEpiColSplit) {

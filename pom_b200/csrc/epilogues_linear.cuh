@@ -1,0 +1,120 @@
+// Epilogue of the linear operator on the tcgen05 GEMM engine: y = act(acc + bias) + residual, and, for a backward pass,
+// the slope act'(acc + bias) beside it.
+//
+// The slope is kept instead of the pre-activation: both cost one bf16 per element, but with the slope the backward pass
+// is a product (dz = dy * slope) where the pre-activation would need the derivative again from its rounded value.
+// Rounding the slope to bf16 (half a step, 2^-9 of its value) puts the same relative error into dz as rounding dz itself,
+// which the tensor cores need anyway.
+#pragma once
+#include "epilogues.cuh"
+#include "linear_math.cuh"
+
+namespace pomk {
+
+template <bool RES>
+struct EpiLinear {
+  struct Params {
+    const void* bias;  // (N) bf16 or fp32, or null
+    int bias_f32;
+    int act;
+    int save_slope;  // maps.out0 = slope; maps.out1 = y; maps.in0 = residual
+  };
+  static constexpr int kSmemBytes = 2 * 256 * 4;  // double-buffered bias
+  // per warp: [slope or y][y], with a residual [residual in][y][slope]
+  static constexpr int kStageBytes = RES ? 6144 : 4096;
+  static constexpr bool kStager = false;
+  template <int BN>
+  static constexpr int smem_bytes() { return kSmemBytes; }
+
+  static __device__ __forceinline__ void fetch(const EpiMaps& maps, const TileCtx& t, EpiIO& io, int quarter, int lane,
+                                               int col) {
+    if (lane == 0) {
+      mbar_expect_tx(io.bar, 32 * 64);
+      tma_load_3d(io.buf0, &maps.in0, io.bar, col, t.row0 + quarter * 32, t.b);
+    }
+  }
+
+  template <int BN>
+  static __device__ __forceinline__ void prologue(const Params& p, const EpiMaps& maps, const GemmGeom& g,
+                                                  const TileCtx& t, int warp_in_epi, int epi_tid, float* scratch,
+                                                  EpiIO& io, int iter) {
+    if constexpr (RES) {
+      const int half = warp_in_epi >> 2, quarter = (warp_in_epi + 2) & 3;
+      const int col = t.col0 + half * 32;
+      if (col < g.n_cols) fetch(maps, t, io, quarter, epi_tid & 31, col);
+    }
+    float* cst = scratch + (iter & 1) * 256;
+    for (int j = epi_tid; j < BN; j += kEpiThreads) {
+      const int col = t.col0 + j;
+      float v = 0.f;
+      if (p.bias && col < g.n_cols)
+        v = p.bias_f32 ? __ldg(static_cast<const float*>(p.bias) + col)
+                       : __bfloat162float(__ldg(static_cast<const __nv_bfloat16*>(p.bias) + col));
+      cst[j] = v;
+    }
+    named_bar_sync(kEpiBarrier, kEpiThreads);
+  }
+
+  template <int BN>
+  static __device__ __forceinline__ void run(const Params& p, const EpiMaps& maps, const GemmGeom& g, const TileCtx& t,
+                                             uint32_t tmem_acc, int quarter, int lane, int half, int, float* scratch,
+                                             EpiIO& io, int iter) {
+    const float* cst = scratch + (iter & 1) * 256;
+    const int y = t.row0 + quarter * 32;
+    uint8_t* const base = io.buf0;
+    // the alternation starts anew with every tile, and a tile may have an odd number of chunks
+    if (lane == 0) bulk_wait_read<0>();
+    int flip = 0;
+    bool alive = true;
+#pragma unroll 1
+    for (int c = half; c < BN / 32; c += kEpiColSplit) {
+      const int col = t.col0 + c * 32;
+      if (col >= g.n_cols) break;  // warp-uniform; the load of this chunk was not started either
+      float v[32];
+      uint32_t pk[16];
+      tmem_ld32(tmem_acc + c * 32, v);
+      tmem_ld_wait();
+#pragma unroll
+      for (int i = 0; i < 32; i += 4) {
+        const float4 b = *reinterpret_cast<const float4*>(cst + c * 32 + i);
+        v[i] += b.x, v[i + 1] += b.y, v[i + 2] += b.z, v[i + 3] += b.w;
+      }
+      if (p.save_slope) {
+        uint32_t ps[16];
+#pragma unroll
+        for (int i = 0; i < 32; i += 2) {
+          float s0, s1;
+          v[i] = linear_act<true>(p.act, v[i], s0);
+          v[i + 1] = linear_act<true>(p.act, v[i + 1], s1);
+          ps[i / 2] = pack_bf16x2(s0, s1);
+        }
+        if (t.rows_valid > 0) store_block<1>(RES ? base + 4096 : base, &maps.out0, ps, lane, col, y, t.b);
+      } else {
+        float none;
+#pragma unroll
+        for (int i = 0; i < 32; ++i) v[i] = linear_act<false>(p.act, v[i], none);
+      }
+      if constexpr (RES) {
+        float r[32];
+        if (alive) alive = mbar_wait(io.bar, io.load_phase, io.abort_flag, io.status, kStatusEpilogueTimeout);
+        alive = __all_sync(0xffffffffu, alive);
+        io.load_phase ^= 1u;
+        read_block(base, lane, r);
+#pragma unroll
+        for (int i = 0; i < 32; ++i) v[i] += r[i];
+        __syncwarp();  // every lane has its residual row: the block may be refilled
+        const int ncol = t.col0 + (c + kEpiColSplit) * 32;
+        if (alive && c + kEpiColSplit < BN / 32 && ncol < g.n_cols) fetch(maps, t, io, quarter, lane, ncol);
+      }
+      pack32(v, pk);
+      if (t.rows_valid > 0) {
+        // with a slope the two stores use one block each; without one, y alternates between two blocks
+        uint8_t* out = RES ? base + (p.save_slope || !flip ? 2048 : 4096) : (p.save_slope || flip ? base + 2048 : base);
+        store_block<1>(out, &maps.out1, pk, lane, col, y, t.b);
+      }
+      flip ^= 1;
+    }
+  }
+};
+
+}  // namespace pomk

@@ -16,7 +16,10 @@ std::atomic<int> g_gemm_mode{0};
 
 namespace pomh {
 
-int gemm_bf16_dead_k(const pom_gemm_args* a, const float* tile_weight, int dead_k, int* status, cudaStream_t st) {
+namespace {
+
+// `slabs` > 1: fp32 output, the K splits' sums side by side (M * ldc elements apart).
+int gemm_bf16_any(const pom_gemm_args* a, const float* tile_weight, int dead_k, int slabs, int* status, cudaStream_t st) {
   if (!a || !a->C) return POM_ERR_NULL;
   Operands o{a->A, a->Bm, a->M, a->N, a->K, a->lda, a->ldb, a->batches, a->a_mn_major != 0, a->b_mn_major != 0};
   o.a_batch_stride = a->a_batch_stride;
@@ -37,12 +40,14 @@ int gemm_bf16_dead_k(const pom_gemm_args* a, const float* tile_weight, int dead_
     if (split > 1) return POM_ERR_UNSUPPORTED;
     split = 1;
   }
-  const TilePlan plan = pick_plan(o, true, a->out_mode == POM_OUT_F32_ACCUM && a->split_k == 0);
+  if (slabs > 1) split = slabs;
+  const TilePlan plan = pick_plan(o, true, slabs > 0 || (a->out_mode == POM_OUT_F32_ACCUM && a->split_k == 0));
   if (split == 0) split = pick_split(plan_units(o, plan), ceil_div(a->K, kBK), plan.pair ? sm_count() / 2 : sm_count());
   EpiStore::Params ep;
   ep.C = a->C;
   ep.ldc = a->ldc;
   ep.batch_stride = a->c_batch_stride ? a->c_batch_stride : a->M * a->ldc;
+  ep.split_stride = slabs > 1 ? a->M * a->ldc : 0;
   if (a->out_mode == POM_OUT_BF16 && a->c_batch_stride % 8) return POM_ERR_BAD_STRIDE;
   if (a->residual && a->c_batch_stride) return POM_ERR_UNSUPPORTED;
   ep.mode = a->out_mode;
@@ -57,6 +62,25 @@ int gemm_bf16_dead_k(const pom_gemm_args* a, const float* tile_weight, int dead_
       (rc = make_io_map(&maps.out0, a->C, a->N, a->M, a->batches, a->ldc, a->c_batch_stride)))
     return rc;
   return run_plan_any_major<EpiStore>(plan, o, split, maps, ep, status, st);
+}
+
+}  // namespace
+
+int gemm_bf16_dead_k(const pom_gemm_args* a, const float* tile_weight, int dead_k, int* status, cudaStream_t st) {
+  return gemm_bf16_any(a, tile_weight, dead_k, 0, status, st);
+}
+
+int gemm_bf16_slabs(int64_t M, int64_t N, int64_t K, bool a_mn, bool b_mn) {
+  const Operands o{nullptr, nullptr, M, N, K, 0, 0, 1, a_mn, b_mn};
+  const TilePlan plan = pick_plan(o, true, true);
+  const long long kb = ceil_div(K, kBK);
+  const int split = pick_split(plan_units(o, plan), kb, plan.pair ? sm_count() / 2 : sm_count());
+  return static_cast<int>(ceil_div(kb, ceil_div(kb, split)));  // as make_geom: no empty split
+}
+
+int gemm_bf16_slabs(const pom_gemm_args* a, int slabs, int* status, cudaStream_t st) {
+  if (!a || slabs < 1 || (slabs > 1 && a->out_mode != POM_OUT_F32)) return POM_ERR_UNSUPPORTED;
+  return gemm_bf16_any(a, nullptr, 0, slabs, status, st);
 }
 
 }  // namespace pomh

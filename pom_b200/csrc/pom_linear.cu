@@ -1,0 +1,493 @@
+// The linear operator: y = act(x W^T + bias) + residual, and its backward pass.
+//
+//   forward   z = x W^T + bias, y = act(z) + residual, slope = act'(z) (kept for a backward pass)
+//   backward  dz = dy * slope;  dx = dz W;  dW = dz^T x;  dbias = sum of dz over the rows;  dresidual = dy
+//
+// bf16, many rows: the tcgen05 GEMM engine with EpiLinear.  Few rows: linear_few_*_kernel, which reads the weight once
+// and spreads it over all SMs.  float32 with many rows: the caller runs pom_gemm_f32 / pom_gemm_f32_planes and
+// pom_linear_epilogue.  Sums are fp32; nothing here is summed by atomics, so a call gives the same bits every time.
+#include "epilogues_linear.cuh"
+#include "gemm_launch.cuh"
+#include "rows.cuh"
+
+using namespace pomk;
+using namespace pomh;
+
+namespace {
+
+struct FewDev {
+  const void *x, *w, *bias, *residual;
+  void *y, *slope;
+  long long ldx, ldw, ldr, ldy, ld_slope;
+  int M, N, K, act, bias_f32;
+};
+
+__device__ __forceinline__ void mma_bf16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                         uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ float few_bias(const FewDev& a, int n) {
+  if (!a.bias) return 0.f;
+  return a.bias_f32 ? __ldg(static_cast<const float*>(a.bias) + n)
+                    : __bfloat162float(__ldg(static_cast<const __nv_bfloat16*>(a.bias) + n));
+}
+
+// bias, activation, residual and stores of one output value.
+template <class T>
+__device__ __forceinline__ void few_finish(const FewDev& a, int row, int n, float z) {
+  Piece<T, 1> p;
+  z += few_bias(a, n);
+  float v[1];
+  if (a.slope) {
+    float s[1];
+    v[0] = linear_act<true>(a.act, z, s[0]);
+    p.set(s);
+    p.st(static_cast<T*>(a.slope) + row * a.ld_slope + n);
+  } else {
+    float none;
+    v[0] = linear_act<false>(a.act, z, none);
+  }
+  if (a.residual) {
+    p.ld(static_cast<const T*>(a.residual) + row * a.ldr + n);
+    v[0] += p.get(0);
+  }
+  p.set(v);
+  p.st(static_cast<T*>(a.y) + row * a.ldy + n);
+}
+
+constexpr int kFewWarps = 8;
+
+// 16 * MT rows per blockIdx.y.  A block owns 8 * NT output columns and reads their weight rows once; its warps take 32-long pieces
+// of K in turn.  Lane (g, t) holds 8 adjacent k of row g of every operand, piece t: which k of the piece the matrix
+// instruction takes for which of its own k does not matter, as long as both operands agree, so the 16 bytes a lane loads
+// are two instructions' fragments as they are.
+template <int MT, int NT>
+__global__ void __launch_bounds__(32 * kFewWarps) linear_few_bf16_kernel(const FewDev a) {
+  constexpr int U = MT == 1 ? 4 : 2;  // pieces in flight
+  __shared__ float red[kFewWarps][16 * MT][8 * NT + 1];
+  griddep_wait();
+  griddep_launch();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const int n0 = blockIdx.x * 8 * NT, m0 = blockIdx.y * 16 * MT;
+  const __nv_bfloat16* w = static_cast<const __nv_bfloat16*>(a.w);
+  const __nv_bfloat16* x = static_cast<const __nv_bfloat16*>(a.x);
+  float c[MT][NT][4];
+#pragma unroll
+  for (int i = 0; i < MT; ++i)
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) c[i][j][e] = 0.f;
+  const uint4 zero = make_uint4(0, 0, 0, 0);
+  for (int kc = warp * 32; kc < a.K; kc += 32 * kFewWarps * U) {
+    uint4 wv[U][NT], xv[U][MT][2];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int k = kc + u * 32 * kFewWarps + t * 8;
+      const bool ok = k < a.K;  // K is a multiple of 8
+#pragma unroll
+      for (int j = 0; j < NT; ++j) {
+        const int n = n0 + j * 8 + g;
+        wv[u][j] = ok && n < a.N ? __ldg(reinterpret_cast<const uint4*>(w + n * a.ldw + k)) : zero;
+      }
+#pragma unroll
+      for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int m = m0 + i * 16 + h * 8 + g;
+          xv[u][i][h] = ok && m < a.M ? __ldg(reinterpret_cast<const uint4*>(x + m * a.ldx + k)) : zero;
+        }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+          mma_bf16(c[i][j], xv[u][i][0].x, xv[u][i][1].x, xv[u][i][0].y, xv[u][i][1].y, wv[u][j].x, wv[u][j].y);
+          mma_bf16(c[i][j], xv[u][i][0].z, xv[u][i][1].z, xv[u][i][0].w, xv[u][i][1].w, wv[u][j].z, wv[u][j].w);
+        }
+  }
+#pragma unroll
+  for (int i = 0; i < MT; ++i)
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+      red[warp][i * 16 + g][j * 8 + 2 * t] = c[i][j][0];
+      red[warp][i * 16 + g][j * 8 + 2 * t + 1] = c[i][j][1];
+      red[warp][i * 16 + g + 8][j * 8 + 2 * t] = c[i][j][2];
+      red[warp][i * 16 + g + 8][j * 8 + 2 * t + 1] = c[i][j][3];
+    }
+  __syncthreads();
+  for (int i = threadIdx.x; i < 16 * MT * 8 * NT; i += 32 * kFewWarps) {
+    const int m = i / (8 * NT), n = i - m * (8 * NT);
+    if (m0 + m >= a.M || n0 + n >= a.N) continue;
+    float z = 0.f;
+#pragma unroll
+    for (int q = 0; q < kFewWarps; ++q) z += red[q][m][n];
+    few_finish<__nv_bfloat16>(a, m0 + m, n0 + n, z);
+  }
+}
+
+// float32, up to MR rows: a block owns 8 columns, lane (ng, kq) the 4 adjacent k of piece kq for columns ng and ng + 4.
+template <int MR>
+__global__ void __launch_bounds__(32 * kFewWarps) linear_few_f32_kernel(const FewDev a) {
+  constexpr int U = MR <= 4 ? 4 : 2;
+  __shared__ float red[kFewWarps][MR][8];
+  griddep_wait();
+  griddep_launch();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, kq = lane & 7, ng = lane >> 3;
+  const int n0 = blockIdx.x * 8;
+  const float* w = static_cast<const float*>(a.w);
+  const float* x = static_cast<const float*>(a.x);
+  float c[MR][2];
+#pragma unroll
+  for (int m = 0; m < MR; ++m) c[m][0] = c[m][1] = 0.f;
+  const float4 zero = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int kc = warp * 32; kc < a.K; kc += 32 * kFewWarps * U) {
+    float4 wv[U][2];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int k = kc + u * 32 * kFewWarps + kq * 4;
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const int n = n0 + ng + 4 * j;
+        wv[u][j] = k < a.K && n < a.N ? __ldg(reinterpret_cast<const float4*>(w + n * a.ldw + k)) : zero;
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int k = kc + u * 32 * kFewWarps + kq * 4;
+#pragma unroll
+      for (int m = 0; m < MR; ++m) {
+        const float4 v = k < a.K && m < a.M ? __ldg(reinterpret_cast<const float4*>(x + m * a.ldx + k)) : zero;
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+          c[m][j] = fmaf(v.w, wv[u][j].w, fmaf(v.z, wv[u][j].z, fmaf(v.y, wv[u][j].y, fmaf(v.x, wv[u][j].x, c[m][j]))));
+      }
+    }
+  }
+#pragma unroll
+  for (int m = 0; m < MR; ++m)
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+#pragma unroll
+      for (int o = 4; o; o >>= 1) c[m][j] += __shfl_xor_sync(0xffffffffu, c[m][j], o);
+      if (kq == 0) red[warp][m][ng + 4 * j] = c[m][j];
+    }
+  __syncthreads();
+  for (int i = threadIdx.x; i < MR * 8; i += 32 * kFewWarps) {
+    const int m = i >> 3, n = i & 7;
+    if (m >= a.M || n0 + n >= a.N) continue;
+    float z = 0.f;
+#pragma unroll
+    for (int q = 0; q < kFewWarps; ++q) z += red[q][m][n];
+    few_finish<float>(a, m, n0 + n, z);
+  }
+}
+
+// y = act(z + bias) + residual, elementwise over (M, N); y may be z itself.  VEC adjacent columns per thread.
+template <class T, int VEC>
+__global__ void __launch_bounds__(256) linear_epilogue_kernel(const FewDev a, const T* z, long long ldz, long long M) {
+  griddep_wait();
+  griddep_launch();
+  const int per_row = a.N / VEC;
+  const long long total = M * per_row;
+  for (long long i = blockIdx.x * 256ll + threadIdx.x; i < total; i += gridDim.x * 256ll) {
+    const long long r = i / per_row;
+    const int c = static_cast<int>(i - r * per_row) * VEC;
+    Piece<T, VEC> p, q;
+    p.raw = *reinterpret_cast<const typename Piece<T, VEC>::R*>(z + r * ldz + c);  // may alias y: no read-only path
+    float v[VEC], s[VEC];
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) v[e] = linear_act<true>(a.act, p.get(e) + few_bias(a, c + e), s[e]);
+    if (a.slope) {
+      q.set(s);
+      q.st(static_cast<T*>(a.slope) + r * a.ld_slope + c);
+    }
+    if (a.residual) {
+      q.ld(static_cast<const T*>(a.residual) + r * a.ldr + c);
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) v[e] += q.get(e);
+    }
+    p.set(v);
+    p.st(static_cast<T*>(a.y) + r * a.ldy + c);
+  }
+}
+
+// dz = dy * slope (no slope: dz = dy, which is not written) and the column sums of dz over the block's rows.
+// Block = 32 column lanes of VEC columns x 8 row lanes; grid = (column blocks, row chunks).
+template <class T, int VEC>
+__global__ void __launch_bounds__(256) linear_dz_kernel(const T* __restrict__ dy, long long ld_dy, const T* __restrict__ slope,
+                                                        T* __restrict__ dz, float* __restrict__ partial, long long M, int N,
+                                                        int chunk) {
+  __shared__ float sm[8][32 * VEC + 1];
+  griddep_wait();
+  griddep_launch();
+  const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
+  const int c = (blockIdx.x * 32 + tx) * VEC;
+  const long long r0 = static_cast<long long>(blockIdx.y) * chunk;
+  const long long r1 = r0 + chunk < M ? r0 + chunk : M;
+  float acc[VEC];
+#pragma unroll
+  for (int e = 0; e < VEC; ++e) acc[e] = 0.f;
+  if (c < N) {
+    constexpr int U = 4;
+    for (long long r = r0 + ty; r < r1; r += 8 * U) {
+      Piece<T, VEC> g[U], s[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (r + 8 * u < r1) {
+          g[u].ld(dy + (r + 8 * u) * ld_dy + c);
+          if (slope) s[u].ld(slope + (r + 8 * u) * N + c);
+        }
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (r + 8 * u < r1) {
+          float v[VEC];
+#pragma unroll
+          for (int e = 0; e < VEC; ++e) {
+            v[e] = slope ? g[u].get(e) * s[u].get(e) : g[u].get(e);
+            acc[e] += v[e];
+          }
+          if (slope) {
+            g[u].set(v);
+            g[u].st(dz + (r + 8 * u) * N + c);
+          }
+        }
+    }
+  }
+  if (!partial) return;
+#pragma unroll
+  for (int e = 0; e < VEC; ++e) sm[ty][tx * VEC + e] = acc[e];
+  __syncthreads();
+  for (int i = threadIdx.x; i < 32 * VEC; i += 256) {
+    const int col = blockIdx.x * 32 * VEC + i;
+    if (col >= N) continue;
+    float s = 0.f;
+#pragma unroll
+    for (int q = 0; q < 8; ++q) s += sm[q][i];
+    partial[static_cast<long long>(blockIdx.y) * N + col] = s;
+  }
+}
+
+// out = sum of the slabs, in their order, in the type T.
+template <class T>
+__global__ void __launch_bounds__(256) linear_slabs_kernel(const float* __restrict__ slabs, int count, long long each,
+                                                           T* __restrict__ out) {
+  griddep_wait();
+  griddep_launch();
+  for (long long i = (blockIdx.x * 256ll + threadIdx.x) * 4; i < each; i += gridDim.x * 1024ll) {
+    float4 s = __ldg(reinterpret_cast<const float4*>(slabs + i));
+    for (int k = 1; k < count; ++k) {
+      const float4 v = __ldg(reinterpret_cast<const float4*>(slabs + k * each + i));
+      s.x += v.x, s.y += v.y, s.z += v.z, s.w += v.w;
+    }
+    Piece<T, 4> p;
+    const float v[4] = {s.x, s.y, s.z, s.w};
+    p.set(v);
+    p.st(out + i);
+  }
+}
+
+int launched(cudaError_t e) {
+  if (e != cudaSuccess) {
+    (void)cudaGetLastError();
+    return POM_ERR_CUDA;
+  }
+  count_launch();
+  return POM_OK;
+}
+
+FewDev few_dev(const pom_linear_args* a) {
+  FewDev d;
+  d.x = a->x, d.w = a->w, d.bias = a->bias, d.residual = a->residual;
+  d.y = a->y, d.slope = a->slope;
+  d.ldx = a->ldx, d.ldw = a->ldw, d.ldr = a->ldr, d.ldy = a->ldy, d.ld_slope = a->N;
+  d.M = static_cast<int>(a->M < INT32_MAX ? a->M : INT32_MAX), d.N = static_cast<int>(a->N), d.K = static_cast<int>(a->K);
+  d.act = a->act, d.bias_f32 = a->bias_dtype == POM_F32;
+  return d;
+}
+
+int check_linear(const pom_linear_args* a) {
+  if (!a) return POM_ERR_NULL;
+  if (a->M <= 0 || a->N <= 0 || a->K <= 0) return POM_ERR_BAD_SHAPE;
+  if (a->M > INT32_MAX || a->N > INT32_MAX || a->K > INT32_MAX) return POM_ERR_TOO_LARGE;
+  if (a->dtype != POM_BF16 && a->dtype != POM_F32) return POM_ERR_UNSUPPORTED;
+  if (a->bias_dtype != POM_BF16 && a->bias_dtype != POM_F32) return POM_ERR_UNSUPPORTED;
+  if (a->act < POM_ACT_NONE || a->act > POM_ACT_RELU) return POM_ERR_UNSUPPORTED;
+  return POM_OK;
+}
+
+constexpr int kFewRowsBf16 = 64, kFewRowsF32 = 16;
+
+template <int MT>
+int launch_few_bf16(const FewDev& d, cudaStream_t st) {
+  const unsigned rows = static_cast<unsigned>(ceil_div(d.M, 16 * MT));
+  // two column tiles per block once that still gives every SM a block: x is read half as often
+  if (d.N >= 16 * sm_count())
+    return launched(launch_pdl(linear_few_bf16_kernel<MT, 2>, dim3(static_cast<unsigned>(ceil_div(d.N, 16)), rows), dim3(32 * kFewWarps), 0, st, d));
+  return launched(launch_pdl(linear_few_bf16_kernel<MT, 1>, dim3(static_cast<unsigned>(ceil_div(d.N, 8)), rows), dim3(32 * kFewWarps), 0, st, d));
+}
+
+template <int MR>
+int launch_few_f32(const FewDev& d, cudaStream_t st) {
+  return launched(launch_pdl(linear_few_f32_kernel<MR>, dim3(static_cast<unsigned>(ceil_div(d.N, 8))), dim3(32 * kFewWarps), 0, st, d));
+}
+
+// Row chunks of linear_dz_kernel: about eight blocks per SM, at least 32 rows each.
+int dz_chunk(int64_t M, int64_t N, int vec) {
+  const int64_t cols = ceil_div(N, 32 * vec), want = ceil_div(8ll * sm_count(), cols);
+  int64_t rows = ceil_div(ceil_div(M, want), 32) * 32;
+  if (ceil_div(M, rows) > 65535) rows = ceil_div(ceil_div(M, 65535), 32) * 32;
+  return static_cast<int>(rows);
+}
+
+struct BwdPlan {
+  int vec, chunk, chunks, slabs;
+  uint64_t dz, partial, slab, total;  // byte offsets into the workspace
+};
+
+BwdPlan bwd_plan(const pom_linear_args* a) {
+  BwdPlan p{};
+  const int per = a->dtype == POM_BF16 ? 8 : 4;
+  p.vec = a->N % per || a->ld_dy % per || !aligned16(a->dy) ? 1 : per;
+  p.chunk = dz_chunk(a->M, a->N, p.vec);
+  p.chunks = static_cast<int>(ceil_div(a->M, p.chunk));
+  p.slabs = a->dtype == POM_BF16 && a->dw ? gemm_bf16_slabs(a->N, a->K, a->M, true, true) : 1;
+  auto up = [](uint64_t v) { return (v + 255) / 256 * 256; };
+  uint64_t at = 0;
+  p.dz = at;
+  if (a->slope && !a->dz) at = up(at + static_cast<uint64_t>(a->M) * a->N * (a->dtype == POM_BF16 ? 2 : 4));
+  p.partial = at;
+  if (a->dbias) at = up(at + static_cast<uint64_t>(p.chunks) * a->N * 4);
+  p.slab = at;
+  if (p.slabs > 1) at = up(at + static_cast<uint64_t>(p.slabs) * a->N * a->K * 4);
+  p.total = at;
+  return p;
+}
+
+// dz (where there is a slope) and dbias.
+int dz_and_bias(const pom_linear_args* a, const BwdPlan& p, void* dz, cudaStream_t st) {
+  if (!a->slope && !a->dbias) return POM_OK;
+  float* partial = a->dbias ? reinterpret_cast<float*>(static_cast<char*>(a->workspace) + p.partial) : nullptr;
+  const dim3 grid(static_cast<unsigned>(ceil_div(a->N, 32 * p.vec)), static_cast<unsigned>(p.chunks));
+  const long long M = a->M, ld = a->ld_dy;
+  const int N = static_cast<int>(a->N);
+#define POM_DZ(T, V)                                                                                                    \
+  launched(launch_pdl(linear_dz_kernel<T, V>, grid, dim3(256), 0, st, static_cast<const T*>(a->dy), ld,                 \
+                      static_cast<const T*>(a->slope), static_cast<T*>(dz), partial, M, N, p.chunk))
+  int rc = a->dtype == POM_BF16 ? (p.vec == 8 ? POM_DZ(__nv_bfloat16, 8) : POM_DZ(__nv_bfloat16, 1))
+                                : (p.vec == 4 ? POM_DZ(float, 4) : POM_DZ(float, 1));
+#undef POM_DZ
+  if (rc || !partial) return rc;
+  return sum_rows(partial, p.chunks, N, N, a->bias_dtype, a->dbias, nullptr, st);
+}
+
+}  // namespace
+
+extern "C" {
+
+int pom_linear_few_rows(const pom_linear_args* a) {
+  if (check_linear(a)) return 0;
+  const int per = a->dtype == POM_BF16 ? 8 : 4;
+  return a->M <= (a->dtype == POM_BF16 ? kFewRowsBf16 : kFewRowsF32) && a->K % per == 0 && a->ldx % per == 0 &&
+         a->ldw % per == 0 && aligned16(a->x) && aligned16(a->w);
+}
+
+int pom_linear_fwd(const pom_linear_args* a, int* status, void* stream) {
+  int rc = check_linear(a);
+  if (rc) return rc;
+  if (!a->x || !a->w || !a->y) return POM_ERR_NULL;
+  if (a->ldx < a->K || a->ldw < a->K || a->ldy < a->N || (a->residual && a->ldr < a->N)) return POM_ERR_BAD_STRIDE;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (pom_linear_few_rows(a)) {
+    const FewDev d = few_dev(a);
+    if (a->dtype == POM_BF16) {
+      return a->M <= 16 ? launch_few_bf16<1>(d, st) : launch_few_bf16<2>(d, st);
+    }
+    if (a->M == 1) return launch_few_f32<1>(d, st);
+    if (a->M <= 4) return launch_few_f32<4>(d, st);
+    if (a->M <= 8) return launch_few_f32<8>(d, st);
+    return launch_few_f32<16>(d, st);
+  }
+  if (a->dtype != POM_BF16) return POM_ERR_UNSUPPORTED;  // pom_gemm_f32* and pom_linear_epilogue
+  Operands o{a->x, a->w, a->M, a->N, a->K, a->ldx, a->ldw, 1, false, false};
+  if ((rc = check_operands(o))) return rc;
+  EpiMaps maps{};
+  if (a->slope && (rc = make_io_map(&maps.out0, a->slope, a->N, a->M, 1, a->N))) return rc;
+  if ((rc = make_io_map(&maps.out1, a->y, a->N, a->M, 1, a->ldy))) return rc;
+  if (a->residual) {
+    if ((rc = make_io_map(&maps.in0, a->residual, a->N, a->M, 1, a->ldr))) return rc;
+    const EpiLinear<true>::Params ep{a->bias, a->bias_dtype == POM_F32, a->act, a->slope != nullptr};
+    return run_plan<false, false, EpiLinear<true>>(pick_plan(o, true), o, 1, maps, ep, status, st);
+  }
+  const EpiLinear<false>::Params ep{a->bias, a->bias_dtype == POM_F32, a->act, a->slope != nullptr};
+  return run_plan<false, false, EpiLinear<false>>(pick_plan(o, true), o, 1, maps, ep, status, st);
+}
+
+int pom_linear_epilogue(const pom_linear_args* a, const float* z, int64_t ldz, void* stream) {
+  int rc = check_linear(a);
+  if (rc) return rc;
+  if (!z || !a->y) return POM_ERR_NULL;
+  if (a->dtype != POM_F32) return POM_ERR_UNSUPPORTED;
+  if (ldz < a->N || a->ldy < a->N || (a->residual && a->ldr < a->N)) return POM_ERR_BAD_STRIDE;
+  const FewDev d = few_dev(a);
+  const bool wide = a->N % 4 == 0 && ldz % 4 == 0 && a->ldy % 4 == 0 && aligned16(z) && aligned16(a->y) &&
+                    aligned16(a->slope) && (!a->residual || (a->ldr % 4 == 0 && aligned16(a->residual)));
+  const int64_t want = ceil_div(a->M * (a->N / (wide ? 4 : 1)), 256), cap = 16ll * sm_count();
+  const dim3 grid(static_cast<unsigned>(want < cap ? want : cap));
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const long long ld = ldz, M = a->M;
+  return wide ? launched(launch_pdl(linear_epilogue_kernel<float, 4>, grid, dim3(256), 0, st, d, z, ld, M))
+              : launched(launch_pdl(linear_epilogue_kernel<float, 1>, grid, dim3(256), 0, st, d, z, ld, M));
+}
+
+uint64_t pom_linear_bwd_workspace(const pom_linear_args* a) { return check_linear(a) ? 0 : bwd_plan(a).total; }
+
+int pom_linear_bwd(const pom_linear_args* a, int* status, void* stream) {
+  int rc = check_linear(a);
+  if (rc) return rc;
+  if (!a->dy || (a->dw && !a->x) || (a->dx && !a->w)) return POM_ERR_NULL;
+  if (a->ld_dy < a->N || (a->dx && a->ldw < a->K) || (a->dw && a->ldx < a->K)) return POM_ERR_BAD_STRIDE;
+  const BwdPlan p = bwd_plan(a);
+  if (p.total && !a->workspace) return POM_ERR_NULL;
+  if (!aligned16(a->workspace) || !aligned16(a->dz)) return POM_ERR_BAD_ALIGN;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  char* ws = static_cast<char*>(a->workspace);
+  void* own_dz = a->dz ? a->dz : ws + p.dz;
+  if ((rc = dz_and_bias(a, p, own_dz, st))) return rc;
+  if (a->dtype != POM_BF16) return a->dx || a->dw ? POM_ERR_UNSUPPORTED : POM_OK;
+  const void* dz = a->slope ? own_dz : a->dy;
+  const int64_t ld_dz = a->slope ? a->N : a->ld_dy;
+  pom_gemm_args g{};
+  g.batches = 1, g.split_k = 1, g.alpha = 1.f;
+  if (a->dw) {
+    float* slabs = reinterpret_cast<float*>(ws + p.slab);
+    g.A = dz, g.Bm = a->x, g.C = p.slabs > 1 ? static_cast<void*>(slabs) : a->dw;
+    g.M = a->N, g.N = a->K, g.K = a->M;
+    g.lda = ld_dz, g.ldb = a->ldx, g.ldc = a->K;
+    g.a_mn_major = g.b_mn_major = 1;
+    g.out_mode = p.slabs > 1 ? POM_OUT_F32 : POM_OUT_BF16;
+    if ((rc = gemm_bf16_slabs(&g, p.slabs, status, st))) return rc;
+    if (p.slabs > 1) {
+      const int64_t each = a->N * a->K, want = ceil_div(each, 1024), cap = 8ll * sm_count();
+      if ((rc = launched(launch_pdl(linear_slabs_kernel<__nv_bfloat16>, dim3(static_cast<unsigned>(want < cap ? want : cap)), dim3(256), 0,
+                                    st, static_cast<const float*>(slabs), p.slabs, static_cast<long long>(each),
+                                    static_cast<__nv_bfloat16*>(a->dw)))))
+        return rc;
+    }
+  }
+  if (a->dx) {
+    g.A = dz, g.Bm = a->w, g.C = a->dx;
+    g.M = a->M, g.N = a->K, g.K = a->N;
+    g.lda = ld_dz, g.ldb = a->ldw, g.ldc = a->K;
+    g.a_mn_major = 0, g.b_mn_major = 1;
+    g.out_mode = POM_OUT_BF16;
+    if ((rc = pom_gemm_bf16(&g, status, st))) return rc;
+  }
+  return check_launch();
+}
+}  // extern "C"

@@ -1,0 +1,198 @@
+// Rotary positions of one to four axes (time, height, width, ...).
+//
+// The channels of x (B, N, H, D) are cut into one section per axis, 2 s_a channels wide and in the order of the axes;
+// channel k of a section is paired with channel k + s_a, and the pair is turned by the angle whose cosine and sine stand
+// in row position_a, column k of the axis' table:
+//     y[k] = x[k] cos - x[k + s] sin        y[k + s] = x[k] sin + x[k + s] cos
+// The transpose (the backward pass) turns the other way.  Channels behind the last section are copied.
+//
+// A thread owns VEC pairs (16 bytes on either side of the pairing where alignment allows) of one token and walks the
+// heads, so that its cosines and sines are read once for all of them.
+#include <limits.h>
+#include <initializer_list>
+#include "rows.cuh"
+
+using namespace pomk;
+using namespace pomh;
+
+namespace {
+
+constexpr int kMaxAxes = POM_ROPE_MAX_AXES;
+
+struct AxesDev {
+  const void* x;
+  void* y;
+  const long long* pos;  // (N, axes), or (B, N, axes)
+  const float* cos[kMaxAxes];
+  const float* sin[kMaxAxes];
+  int len[kMaxAxes], pairs[kMaxAxes];
+  long long xs_b, xs_n, xs_h;  // strides of x; y is contiguous
+  long long B, N;
+  int H, D, axes, units, pair_units;
+  int pos_per_sample;
+  float sign;
+};
+
+template <class T, int VEC>
+__global__ void __launch_bounds__(256) rope_axes_kernel(const AxesDev a) {
+  griddep_wait();
+  griddep_launch();
+  const long long total = a.B * a.N * a.units;
+  for (long long i = blockIdx.x * 256ll + threadIdx.x; i < total; i += gridDim.x * 256ll) {
+    const long long tok = i / a.units;
+    int u = static_cast<int>(i - tok * a.units);
+    const long long b = tok / a.N, n = tok - b * a.N;
+    const T* x = static_cast<const T*>(a.x) + b * a.xs_b + n * a.xs_n;
+    T* y = static_cast<T*>(a.y) + tok * a.H * a.D;
+    if (u >= a.pair_units) {  // a copied channel block
+      const int c = a.D - (a.units - u) * VEC;
+      for (int h = 0; h < a.H; ++h) {
+        Piece<T, VEC> p;
+        p.ld(x + h * a.xs_h + c);
+        p.st(y + static_cast<long long>(h) * a.D + c);
+      }
+      continue;
+    }
+    int axis = 0, lo = 0;  // section and its first channel
+    while (u * VEC >= a.pairs[axis]) u -= a.pairs[axis] / VEC, lo += 2 * a.pairs[axis], ++axis;
+    const int s = a.pairs[axis], k = u * VEC;
+    const long long p = __ldg(a.pos + (a.pos_per_sample ? tok : n) * a.axes + axis);
+    float cs[VEC], sn[VEC];
+    if (p >= 0 && p < a.len[axis]) {
+      const float* ct = a.cos[axis] + p * s + k;
+      const float* st = a.sin[axis] + p * s + k;
+      constexpr int F = VEC < 4 ? VEC : 4;
+#pragma unroll
+      for (int e = 0; e < VEC; e += F) {
+        Piece<float, F> pc, ps;
+        pc.ld(ct + e), ps.ld(st + e);
+#pragma unroll
+        for (int f = 0; f < F; ++f) cs[e + f] = pc.get(f), sn[e + f] = a.sign * ps.get(f);
+      }
+    } else {  // no such row: not a number, and never a read outside the table
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) cs[e] = sn[e] = __int_as_float(0x7fc00000);
+    }
+    for (int h = 0; h < a.H; ++h) {
+      Piece<T, VEC> p1, p2;
+      p1.ld(x + h * a.xs_h + lo + k);
+      p2.ld(x + h * a.xs_h + lo + s + k);
+      float v1[VEC], v2[VEC];
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        const float x1 = p1.get(e), x2 = p2.get(e);
+        v1[e] = x1 * cs[e] - x2 * sn[e];
+        v2[e] = x1 * sn[e] + x2 * cs[e];
+      }
+      p1.set(v1), p2.set(v2);
+      p1.st(y + static_cast<long long>(h) * a.D + lo + k);
+      p2.st(y + static_cast<long long>(h) * a.D + lo + s + k);
+    }
+  }
+}
+
+// Smallest and largest position per axis: info[2 * axis] and info[2 * axis + 1].  One block.
+__global__ void __launch_bounds__(1024) pos_range_kernel(const long long* __restrict__ pos, long long rows, int axes,
+                                                         long long* __restrict__ info) {
+  __shared__ long long s_lo[32], s_hi[32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  for (int c = 0; c < axes; ++c) {
+    long long lo = LLONG_MAX, hi = LLONG_MIN;
+    for (long long i = threadIdx.x; i < rows; i += 1024) {
+      const long long p = __ldg(pos + i * axes + c);
+      lo = p < lo ? p : lo;
+      hi = p > hi ? p : hi;
+    }
+    for (int o = 16; o; o >>= 1) {
+      const long long l = __shfl_xor_sync(0xffffffffu, lo, o), h = __shfl_xor_sync(0xffffffffu, hi, o);
+      lo = l < lo ? l : lo;
+      hi = h > hi ? h : hi;
+    }
+    if (lane == 0) s_lo[warp] = lo, s_hi[warp] = hi;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      for (int w = 1; w < 32; ++w) {
+        lo = s_lo[w] < lo ? s_lo[w] : lo;
+        hi = s_hi[w] > hi ? s_hi[w] : hi;
+      }
+      info[2 * c] = lo, info[2 * c + 1] = hi;
+    }
+    __syncthreads();
+  }
+}
+
+// Pairs per thread: 16 bytes of x where every section, stride and address allows it, else 4 bytes, else one value.
+int axes_vec(const pom_rope_axes_args* a, int wide) {
+  for (int v : {wide, 2}) {
+    bool ok = a->D % v == 0 && a->xs_b % v == 0 && a->xs_n % v == 0 && a->xs_h % v == 0;
+    const uintptr_t xm = static_cast<uintptr_t>(v) * (a->dtype == POM_BF16 ? 2 : 4) - 1;
+    const uintptr_t fm = (v < 4 ? v : 4) * 4 - 1;
+    ok = ok && !((reinterpret_cast<uintptr_t>(a->x) | reinterpret_cast<uintptr_t>(a->y)) & xm);
+    for (int i = 0; i < a->axes; ++i)
+      ok = ok && a->pairs[i] % v == 0 &&
+           !((reinterpret_cast<uintptr_t>(a->cos[i]) | reinterpret_cast<uintptr_t>(a->sin[i])) & fm);
+    if (ok) return v;
+  }
+  return 1;
+}
+
+}  // namespace
+
+extern "C" {
+
+int pom_rope_axes(const pom_rope_axes_args* a, void* stream) {
+  if (!a || !a->x || !a->y || !a->pos) return POM_ERR_NULL;
+  if (a->axes < 1 || a->axes > kMaxAxes) return POM_ERR_UNSUPPORTED;
+  if (a->dtype != POM_BF16 && a->dtype != POM_F32) return POM_ERR_UNSUPPORTED;
+  if (a->B <= 0 || a->N <= 0 || a->H <= 0 || a->D <= 0) return POM_ERR_BAD_SHAPE;
+  if (a->xs_b < 0 || a->xs_n < 0 || a->xs_h < 0) return POM_ERR_BAD_STRIDE;
+  AxesDev d;
+  long long total_pairs = 0;
+  for (int i = 0; i < kMaxAxes; ++i) {
+    d.cos[i] = a->cos[i], d.sin[i] = a->sin[i], d.len[i] = a->len[i], d.pairs[i] = a->pairs[i];
+    if (i >= a->axes) continue;
+    if (!a->cos[i] || !a->sin[i]) return POM_ERR_NULL;
+    if (a->len[i] <= 0 || a->pairs[i] <= 0) return POM_ERR_BAD_SHAPE;
+    total_pairs += a->pairs[i];
+  }
+  if (2 * total_pairs > a->D) return POM_ERR_BAD_SHAPE;
+  const int vec = axes_vec(a, a->dtype == POM_BF16 ? 8 : 4);
+  d.x = a->x, d.y = a->y, d.pos = reinterpret_cast<const long long*>(a->pos);
+  d.xs_b = a->xs_b, d.xs_n = a->xs_n, d.xs_h = a->xs_h;
+  d.B = a->B, d.N = a->N, d.H = a->H, d.D = a->D, d.axes = a->axes;
+  d.pair_units = static_cast<int>(total_pairs / vec);
+  d.units = d.pair_units + static_cast<int>((a->D - 2 * total_pairs) / vec);
+  d.pos_per_sample = a->pos_per_sample;
+  d.sign = a->transpose ? -1.f : 1.f;
+  const int64_t want = ceil_div(a->B * a->N * d.units, 256), cap = 64ll * sm_count();
+  const dim3 grid(static_cast<unsigned>(want < cap ? want : cap));
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  cudaError_t e;
+#define POM_AXES(T, V) e = launch_pdl(rope_axes_kernel<T, V>, grid, dim3(256), 0, st, d)
+  if (a->dtype == POM_BF16) {
+    if (vec == 8) POM_AXES(__nv_bfloat16, 8);
+    else if (vec == 2) POM_AXES(__nv_bfloat16, 2);
+    else POM_AXES(__nv_bfloat16, 1);
+  } else {
+    if (vec == 4) POM_AXES(float, 4);
+    else if (vec == 2) POM_AXES(float, 2);
+    else POM_AXES(float, 1);
+  }
+#undef POM_AXES
+  if (e != cudaSuccess) {
+    (void)cudaGetLastError();
+    return POM_ERR_CUDA;
+  }
+  count_launch();
+  return check_launch();
+}
+
+int pom_pos_range(const int64_t* pos, int64_t rows, int32_t axes, int64_t* info, void* stream) {
+  if (!pos || !info) return POM_ERR_NULL;
+  if (rows <= 0 || axes < 1 || axes > kMaxAxes) return POM_ERR_BAD_SHAPE;
+  pos_range_kernel<<<1, 1024, 0, static_cast<cudaStream_t>(stream)>>>(
+      reinterpret_cast<const long long*>(pos), rows, axes, reinterpret_cast<long long*>(info));
+  count_launch();
+  return check_launch();
+}
+}  // extern "C"

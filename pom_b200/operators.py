@@ -9,6 +9,9 @@ The reference exposes its fused kernels as functions that its tests and benchmar
 and raise the same errors; all of them run on the CUDA operators of this package (there is no CPU path) and
 are differentiable.  The ``*_triton`` names and the ``TRITON_*_AVAILABLE`` flags are kept as aliases so that a
 script written against the reference's modules needs only its import lines changed.
+
+``layer_norm``, ``linear``, ``apply_rope_axes`` and ``precompute_freqs_axes`` (``block_ops.py``) have no counterpart
+there: they are what a residual block around the mixer needs besides it.
 """
 from __future__ import annotations
 
@@ -17,11 +20,13 @@ from typing import Optional
 import torch
 
 from . import _abi, ops
+from .block_ops import apply_rope_axes, layer_norm, linear, precompute_freqs_axes  # noqa: F401
 from .functional import MAX_BATCH, _batch_slices, _f32, _ones, eager_only, on_tensor_device, polynomial_aggregation_
 from .ops import RopeSpec
 
 __all__ = [
-    "pom_activation", "poly_features", "apply_rope_1d", "apply_rope_2d",
+    "pom_activation", "poly_features", "apply_rope_1d", "apply_rope_2d", "apply_rope_axes", "precompute_freqs_axes",
+    "layer_norm", "linear",
     "poly_agg_mean", "poly_agg_causal", "poly_agg_masked", "poly_agg_rope_mean", "poly_agg_rope_causal",
     "poly_agg_mean_triton", "poly_agg_causal_triton", "poly_agg_masked_triton", "poly_agg_rope_mean_triton",
     "poly_agg_rope_causal_triton", "TRITON_AVAILABLE", "TRITON_CAUSAL_AVAILABLE", "TRITON_MASKED_AVAILABLE",

@@ -15,8 +15,8 @@ from typing import Optional, Tuple
 import torch
 
 from . import _abi
-from ._abi import (AggArgs, AggBwdArgs, CtxArgs, GateArgs, GateBwdArgs, GemmArgs, Rope, SelectArgs, SelectBwdArgs,
-                   SelectHeadsArgs, ptr)
+from ._abi import (AggArgs, AggBwdArgs, CtxArgs, GateArgs, GateBwdArgs, GemmArgs, LayerNormArgs, LinearArgs, Rope,
+                   RopeAxesArgs, SelectArgs, SelectBwdArgs, SelectHeadsArgs, ptr)
 
 
 def _require_cuda(*tensors) -> torch.device:
@@ -930,6 +930,211 @@ def zeros_f32(n: int, device) -> torch.Tensor:
     """Flat fp32 buffer of n zeros (allocation by PyTorch, fill by cudaMemsetAsync on the current stream)."""
     out = torch.empty((n,), dtype=torch.float32, device=device)
     _abi.check(_abi.lib().pom_fill_zero(ptr(out), out.numel() * 4, _abi.stream_ptr()), "pom_fill_zero")
+    return out
+
+
+# ---------------------------------------------------------------------------- operators of a residual block
+def rows_of(t: torch.Tensor, align: bool = False):
+    """(tensor, leading dimension): ``t`` as rows of its last dimension, itself where its strides allow, else a copy.
+    ``align``: rows start on 16-byte boundaries (what bulk copies of a bf16 operand need; the width is a multiple of 8)."""
+    w = t.shape[-1]
+    ld = w
+    if not t.is_contiguous():
+        shape, stride = t.shape, t.stride()
+        ok = stride[-1] == 1 or w == 1
+        step = None  # the one stride between consecutive rows; dimensions of size 1 have none
+        for n, s in zip(reversed(shape[:-1]), reversed(stride[:-1])):
+            if n == 1:
+                continue
+            if step is None:
+                step, ld = s * n, s
+            elif s == step:
+                step = s * n
+            else:
+                ok = False
+        if not ok or ld < w or (align and ld % 8):
+            t, ld = t.contiguous(), w
+    if align and t.data_ptr() % 16:
+        t, ld = t.clone(memory_format=torch.contiguous_format), w
+    return t, ld
+
+
+def layer_norm_fwd(x: torch.Tensor, weight: Optional[torch.Tensor], bias: Optional[torch.Tensor], eps: float,
+                   want_stats: bool):
+    """Layer norm over the last dimension: (y, stats), stats (M, 2) fp32 = mean and 1 / sqrt(var + eps) of every row, or
+    None.  ``weight`` and ``bias`` contiguous, of one dtype."""
+    dev = _require_cuda(x, weight, bias)
+    x, ld = rows_of(x)
+    D = x.shape[-1]
+    M = x.numel() // D
+    y = torch.empty(x.shape, dtype=x.dtype, device=dev)
+    stats = torch.empty((M, 2), dtype=torch.float32, device=dev) if want_stats else None
+    if M:
+        a = LayerNormArgs()
+        a.x, a.y, a.M, a.ldx, a.ldy, a.D, a.eps = x.data_ptr(), y.data_ptr(), M, ld, D, D, eps
+        a.dtype = a.wdtype = _abi.dtype_code(x.dtype)
+        if weight is not None:
+            a.weight, a.bias, a.wdtype = weight.data_ptr(), ptr(bias), _abi.dtype_code(weight.dtype)
+        if stats is not None:
+            a.stats = stats.data_ptr()
+        _abi.check(_abi.lib().pom_layer_norm_fwd(C.byref(a), _abi.stream_ptr()), "pom_layer_norm_fwd")
+    return y, stats
+
+
+def layer_norm_bwd(dy: torch.Tensor, x: torch.Tensor, weight: Optional[torch.Tensor], stats: torch.Tensor, *,
+                   want_dx: bool, want_dw: bool, want_db: bool):
+    """(dx, dweight, dbias) of :func:`layer_norm_fwd`; what is not wanted is None."""
+    dev = _require_cuda(dy, x, weight, stats)
+    x, ldx = rows_of(x)
+    dy, ldg = rows_of(dy)
+    D = x.shape[-1]
+    M = x.numel() // D
+    dx = torch.empty(x.shape, dtype=x.dtype, device=dev) if want_dx else None
+    dw = torch.empty_like(weight) if want_dw else None
+    db = torch.empty_like(weight) if want_db else None
+    if M == 0:
+        return dx, dw if dw is None else fill_zero(dw), db if db is None else fill_zero(db)
+    a = LayerNormArgs()
+    a.x, a.dy, a.stats, a.weight = x.data_ptr(), dy.data_ptr(), stats.data_ptr(), ptr(weight)
+    a.dx, a.dweight, a.dbias = ptr(dx), ptr(dw), ptr(db)
+    a.M, a.ldx, a.ld_dy, a.ld_dx, a.D = M, ldx, ldg, D, D
+    a.dtype = _abi.dtype_code(x.dtype)
+    a.wdtype = a.dtype if weight is None else _abi.dtype_code(weight.dtype)
+    L = _abi.lib()
+    if want_dw or want_db:
+        ws = torch.empty((int(L.pom_layer_norm_bwd_workspace(C.byref(a))),), dtype=torch.uint8, device=dev)
+        a.workspace = ws.data_ptr()
+    _abi.check(L.pom_layer_norm_bwd(C.byref(a), _abi.stream_ptr()), "pom_layer_norm_bwd")
+    return dx, dw, db
+
+
+def _linear_args(x, w, bias, act, M, N, K, ldx, ldw) -> LinearArgs:
+    a = LinearArgs()
+    a.x, a.w, a.M, a.N, a.K, a.ldx, a.ldw = x.data_ptr(), w.data_ptr(), M, N, K, ldx, ldw
+    a.act, a.dtype = _abi.ACTIVATIONS[act], _abi.dtype_code(x.dtype)
+    if bias is not None:
+        a.bias, a.bias_dtype = bias.data_ptr(), _abi.dtype_code(bias.dtype)
+    return a
+
+
+def linear_fwd(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor], act: Optional[str],
+               residual: Optional[torch.Tensor], want_slope: bool):
+    """act(x·wᵀ + bias) + residual: (y, slope), slope (M, N) = act'(x·wᵀ + bias) or None.  x (..., K), w (N, K), both bf16
+    (K and N multiples of 8) or both float32; ``bias`` contiguous, bf16 or float32."""
+    dev = _require_cuda(x, w, bias, residual)
+    bf16 = x.dtype == torch.bfloat16
+    x, ldx = rows_of(x, bf16)
+    w, ldw = rows_of(w, bf16)
+    N, K = w.shape
+    M = x.numel() // K
+    y = torch.empty((*x.shape[:-1], N), dtype=x.dtype, device=dev)
+    slope = torch.empty((M, N), dtype=x.dtype, device=dev) if want_slope else None
+    if M == 0:
+        return y, slope
+    a = _linear_args(x, w, bias, act, M, N, K, ldx, ldw)
+    a.y, a.ldy = y.data_ptr(), N
+    if slope is not None:
+        a.slope = slope.data_ptr()
+    if residual is not None:
+        residual, a.ldr = rows_of(residual, bf16)
+        a.residual = residual.data_ptr()
+    L = _abi.lib()
+    if bf16 or L.pom_linear_few_rows(C.byref(a)):
+        _abi.check(L.pom_linear_fwd(C.byref(a), _abi.status_word(dev).data_ptr(), _abi.stream_ptr()), "pom_linear_fwd")
+        return y, slope
+    y2 = y.view(M, N)
+    gemm(x.as_strided((M, K), (ldx, 1)), w.as_strided((N, K), (ldw, 1)), out=y2)
+    if bias is not None or residual is not None or act is not None:
+        _abi.check(L.pom_linear_epilogue(C.byref(a), y.data_ptr(), N, _abi.stream_ptr()), "pom_linear_epilogue")
+    return y, slope
+
+
+def linear_bwd(dy: torch.Tensor, x: torch.Tensor, w: torch.Tensor, slope: Optional[torch.Tensor], *, want_dx: bool,
+               want_dw: bool, bias_dtype: Optional[torch.dtype]):
+    """(dx, dw, dbias) of :func:`linear_fwd` (dbias where ``bias_dtype`` is given); what is not wanted is None."""
+    dev = _require_cuda(dy, x, w, slope)
+    bf16 = x.dtype == torch.bfloat16
+    x, ldx = rows_of(x, bf16)
+    w, ldw = rows_of(w, bf16)
+    N, K = w.shape
+    M = x.numel() // K
+    dx = torch.empty(x.shape, dtype=x.dtype, device=dev) if want_dx else None
+    dw = torch.empty((N, K), dtype=w.dtype, device=dev) if want_dw else None
+    db = torch.empty((N,), dtype=bias_dtype, device=dev) if bias_dtype is not None else None
+    if M == 0:
+        return dx, dw if dw is None else fill_zero(dw), db if db is None else fill_zero(db)
+    dy, ldg = rows_of(dy, bf16)
+    a = _linear_args(x, w, None, None, M, N, K, ldx, ldw)
+    a.dy, a.ld_dy, a.slope, a.dbias = dy.data_ptr(), ldg, ptr(slope), ptr(db)
+    if db is not None:
+        a.bias_dtype = _abi.dtype_code(bias_dtype)
+    dz = None
+    if bf16:
+        a.dx, a.dw = ptr(dx), ptr(dw)
+    elif slope is not None:
+        dz = torch.empty((M, N), dtype=x.dtype, device=dev)
+        a.dz = dz.data_ptr()
+    L = _abi.lib()
+    nbytes = int(L.pom_linear_bwd_workspace(C.byref(a)))
+    if nbytes:
+        ws = torch.empty((nbytes,), dtype=torch.uint8, device=dev)
+        a.workspace = ws.data_ptr()
+    _abi.check(L.pom_linear_bwd(C.byref(a), _abi.status_word(dev).data_ptr(), _abi.stream_ptr()), "pom_linear_bwd")
+    if not bf16:
+        if dz is None:
+            dz = dy.as_strided((M, N), (ldg, 1))
+        planes = F32Planes()  # of dz, which enters both products
+        if want_dw:
+            gemm(dz, x.as_strided((M, K), (ldx, 1)), a_mn=True, b_mn=True, out=dw, a_planes=planes)
+        if want_dx:
+            gemm(dz, w.as_strided((N, K), (ldw, 1)), b_mn=True, out=dx.view(M, K), a_planes=planes)
+    return dx, dw, db
+
+
+def rope_axes(x: torch.Tensor, pos: torch.Tensor, tables, transpose: bool = False) -> torch.Tensor:
+    """Rotation of x (B, N, D) or (B, N, H, D) by positions of several axes (``pom_rope_axes``).  pos (N, A) or (B, N, A)
+    int64 contiguous; ``tables``: one (cos, sin) pair of contiguous fp32 (rows, pairs) tensors per axis."""
+    dev = _require_cuda(x, pos, *(t for cs in tables for t in cs))
+    if x.stride(-1) != 1 and x.shape[-1] > 1:
+        x = x.contiguous()
+    y = torch.empty(x.shape, dtype=x.dtype, device=dev)
+    if y.numel() == 0:
+        return y
+    a = RopeAxesArgs()
+    a.x, a.y, a.pos = x.data_ptr(), y.data_ptr(), pos.data_ptr()
+    for i, (c, s) in enumerate(tables):
+        a.cos[i], a.sin[i], a.len[i], a.pairs[i] = c.data_ptr(), s.data_ptr(), c.shape[0], c.shape[1]
+    # a dimension of size 1 is never stepped over: its stride (PyTorch may report any) must not cost the wide access
+    st = [s if n > 1 else 0 for n, s in zip(x.shape, x.stride())]
+    a.xs_b, a.xs_n, a.xs_h = st[0], st[1], st[2] if x.dim() == 4 else 0
+    a.B, a.N, a.H, a.D = x.shape[0], x.shape[1], x.shape[2] if x.dim() == 4 else 1, x.shape[-1]
+    a.axes, a.dtype = len(tables), _abi.dtype_code(x.dtype)
+    a.pos_per_sample, a.transpose = int(pos.dim() == 3), int(transpose)
+    _abi.check(_abi.lib().pom_rope_axes(C.byref(a), _abi.stream_ptr()), "pom_rope_axes")
+    return y
+
+
+_pos_range_cache = {}
+
+
+def pos_range(pos: torch.Tensor):
+    """(min, max) per column of the (..., A) int64 positions.  One small kernel and a synchronising read the first time a
+    given tensor (object and version) is seen; later calls are answered from a cache, as :func:`rope_pos_info`'s are."""
+    _require_cuda(pos)
+    cacheable = not pos.is_inference()
+    key = id(pos)
+    ent = _pos_range_cache.get(key) if cacheable else None
+    if ent is not None and ent[0]() is pos and ent[1] == pos._version:
+        return ent[2]
+    axes = pos.shape[-1]
+    flat = pos.contiguous()
+    info = torch.empty((2 * axes,), dtype=torch.int64, device=pos.device)
+    _abi.check(_abi.lib().pom_pos_range(flat.data_ptr(), flat.numel() // axes, axes, info.data_ptr(), _abi.stream_ptr()),
+               "pom_pos_range")
+    v = info.cpu().tolist()
+    out = tuple(zip(v[::2], v[1::2]))
+    if cacheable:
+        _pos_range_cache[key] = (weakref.ref(pos, lambda _r, k=key: _pos_range_cache.pop(k, None)), pos._version, out)
     return out
 
 
