@@ -209,11 +209,11 @@ class LinearArgs(C.Structure):
 ROPE_MAX_AXES = 4
 
 
-class RopeAxesArgs(C.Structure):
+class RopeAxesArgs(C.Structure):  # the C arrays cos, sin, len and pairs as single fields, which are cheaper to set
     _fields_ = [
         ("x", C.c_void_p), ("y", C.c_void_p), ("pos", C.c_void_p),
-        ("cos", C.c_void_p * ROPE_MAX_AXES), ("sin", C.c_void_p * ROPE_MAX_AXES),
-        ("len", C.c_int32 * ROPE_MAX_AXES), ("pairs", C.c_int32 * ROPE_MAX_AXES),
+        *[(f"cos{i}", C.c_void_p) for i in range(ROPE_MAX_AXES)], *[(f"sin{i}", C.c_void_p) for i in range(ROPE_MAX_AXES)],
+        *[(f"len{i}", C.c_int32) for i in range(ROPE_MAX_AXES)], *[(f"pairs{i}", C.c_int32) for i in range(ROPE_MAX_AXES)],
         ("xs_b", C.c_int64), ("xs_n", C.c_int64), ("xs_h", C.c_int64),
         ("B", C.c_int64), ("N", C.c_int64),
         ("H", C.c_int32), ("D", C.c_int32), ("axes", C.c_int32), ("dtype", C.c_int32),

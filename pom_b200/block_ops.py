@@ -9,6 +9,7 @@ run.  ``pom_b200.operators`` exports them.
 """
 from __future__ import annotations
 
+import functools
 from typing import Optional, Sequence, Tuple
 
 import torch
@@ -16,7 +17,7 @@ import torch.nn.functional as F
 from torch.autograd.function import once_differentiable
 
 from . import _abi, ops
-from .functional import eager_only, on_tensor_device
+from .functional import eager_only
 
 _any_autocast = getattr(torch._C, "_is_any_autocast_enabled", lambda: True)
 _TYPES = (torch.bfloat16, torch.float32)
@@ -30,8 +31,37 @@ def _check_tokens(x: torch.Tensor, name: str = "x") -> None:
         raise TypeError(f"unsupported dtype {x.dtype} of {name}; use bfloat16 or float32")
 
 
-def _tracked(*tensors) -> bool:
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+
+
+def _entry(fn):
+    """``eager_only`` and a switch to the device of the first argument, as the package's other entry points make it; one
+    wrapper of few steps, because a small call costs the host more than the GPU."""
+
+    @eager_only
+    @functools.wraps(fn)
+    def wrapper(x, *args, **kwargs):
+        if isinstance(x, torch.Tensor):
+            i = x.get_device()
+            if i >= 0 and i != _current_device():
+                with torch.cuda.device(i):
+                    return fn(x, *args, **kwargs)
+        return fn(x, *args, **kwargs)
+
+    return wrapper
+
+
+def _backward(fn):
+    """A backward pass that is differentiable once.  Under ``create_graph`` it goes through ``once_differentiable``, whose
+    outputs refuse a second differentiation; the ordinary case does without that wrapper.  The engine calls it with the
+    device of the forward call current."""
+    checked = once_differentiable(fn)
+
+    @functools.wraps(fn)
+    def wrapper(ctx, g):
+        return checked(ctx, g) if torch.is_grad_enabled() else fn(ctx, g)
+
+    return staticmethod(wrapper)
 
 
 # --------------------------------------------------------------------------- layer norm
@@ -42,9 +72,7 @@ class _LayerNorm(torch.autograd.Function):
         ctx.save_for_backward(x, weight, stats)
         return y
 
-    @staticmethod
-    @once_differentiable
-    @on_tensor_device
+    @_backward
     def backward(ctx, g):
         x, weight, stats = ctx.saved_tensors
         nx, nw, nb, _ = ctx.needs_input_grad
@@ -52,8 +80,7 @@ class _LayerNorm(torch.autograd.Function):
         return dx, dw, db, None
 
 
-@eager_only
-@on_tensor_device
+@_entry
 def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None,
                eps: float = 1e-5) -> torch.Tensor:
     """``(x - mean) / sqrt(var + eps) * weight + bias`` over the last dimension, in x's dtype.
@@ -85,7 +112,8 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
                 bias = bias.to(weight.dtype)
             if not bias.is_contiguous():
                 bias = bias.contiguous()
-    if _tracked(x, weight, bias):
+    if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad) or
+                                    (bias is not None and bias.requires_grad)):
         return _LayerNorm.apply(x, weight, bias, eps)
     return ops.layer_norm_fwd(x, weight, bias, eps, False)[0]
 
@@ -100,9 +128,7 @@ class _Linear(torch.autograd.Function):
         ctx.bias_dtype = bias.dtype if nb else None
         return y
 
-    @staticmethod
-    @once_differentiable
-    @on_tensor_device
+    @_backward
     def backward(ctx, g):
         x, weight, slope = ctx.saved_tensors
         nx, nw, nb, nr, _ = ctx.needs_input_grad
@@ -116,8 +142,7 @@ def _pad8(n: int) -> int:
     return -n % 8
 
 
-@eager_only
-@on_tensor_device
+@_entry
 def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None, *,
            activation: Optional[str] = None, residual: Optional[torch.Tensor] = None) -> torch.Tensor:
     """``activation(x · weightᵀ + bias) + residual`` in one product.
@@ -161,7 +186,8 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] =
         y = linear(F.pad(x, (0, kp)), F.pad(weight, (0, kp, 0, n_pad)), None if bias is None else F.pad(bias, (0, n_pad)),
                    activation=activation, residual=None if residual is None else F.pad(residual, (0, n_pad)))
         return y[..., :N].contiguous() if n_pad else y
-    if _tracked(x, weight, bias, residual):
+    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad) or
+                                    (residual is not None and residual.requires_grad)):
         return _Linear.apply(x, weight, bias, residual, activation)
     return ops.linear_fwd(x, weight, bias, activation, residual, False)[0]
 
@@ -173,15 +199,18 @@ class _RotateAxes(torch.autograd.Function):
         ctx.pos, ctx.tables = pos, tables
         return ops.rope_axes(x, pos, tables)
 
-    @staticmethod
-    @once_differentiable
-    @on_tensor_device
+    @_backward
     def backward(ctx, g):
         return ops.rope_axes(g, ctx.pos, ctx.tables, transpose=True), None, None
 
 
-@eager_only
-@on_tensor_device
+def _f32_on(t: torch.Tensor, device: int, x: torch.Tensor) -> torch.Tensor:
+    if t.dtype == torch.float32 and t.get_device() == device and t.is_contiguous():
+        return t
+    return t.to(device=x.device, dtype=torch.float32).contiguous()
+
+
+@_entry
 def apply_rope_axes(x: torch.Tensor, positions: torch.Tensor, tables: Sequence[Tuple[torch.Tensor, torch.Tensor]], *,
                     validate: bool = True) -> torch.Tensor:
     """Rotary positions of one to four axes, e.g. (time, height, width) of video tokens.
@@ -199,28 +228,30 @@ def apply_rope_axes(x: torch.Tensor, positions: torch.Tensor, tables: Sequence[T
     if not 1 <= len(tables) <= _abi.ROPE_MAX_AXES:
         raise ValueError(f"1 to {_abi.ROPE_MAX_AXES} axes, got {len(tables)}")
     D, axes, width, tabs = x.shape[-1], len(tables), 0, []
-    for i, (cos, sin) in enumerate(tables):
-        if cos.dim() != 2 or cos.shape != sin.shape or 0 in cos.shape:
-            raise ValueError(f"tables[{i}] must be two (rows, pairs) tensors of one shape, got {tuple(cos.shape)} and "
+    device = x.get_device()
+    for cos, sin in tables:
+        shape = cos.shape
+        if len(shape) != 2 or shape != sin.shape or 0 in shape:
+            raise ValueError(f"every table must be two (rows, pairs) tensors of one shape, got {tuple(shape)} and "
                              f"{tuple(sin.shape)}")
-        width += 2 * cos.shape[1]
-        tabs.append(tuple(t if t.dtype == torch.float32 and t.device == x.device and t.is_contiguous()
-                          else t.to(device=x.device, dtype=torch.float32).contiguous() for t in (cos, sin)))
+        width += 2 * shape[1]
+        tabs.append((_f32_on(cos, device, x), _f32_on(sin, device, x)))
     if width > D:
         raise ValueError(f"the axes rotate {width} channels but x has {D}")
     B, N = x.shape[:2]
-    if tuple(positions.shape) not in ((N, axes), (B, N, axes)):
+    if positions.shape != (N, axes) and positions.shape != (B, N, axes):
         raise ValueError(f"positions must have shape ({N}, {axes}) or ({B}, {N}, {axes}), got {tuple(positions.shape)}")
-    if positions.dtype.is_floating_point or positions.dtype == torch.bool:
-        raise TypeError(f"positions must be integers, got {positions.dtype}")
-    if validate and positions.numel():
-        on_gpu = positions if positions.dtype == torch.int64 and positions.device == x.device else \
-            positions.to(device=x.device, dtype=torch.int64)
-        for a, ((lo, hi), (cos, _)) in enumerate(zip(ops.pos_range(on_gpu), tabs)):
+    pos = positions
+    if pos.dtype != torch.int64 or pos.get_device() != device:
+        if pos.dtype.is_floating_point or pos.dtype == torch.bool or pos.dtype.is_complex:
+            raise TypeError(f"positions must be integers, got {pos.dtype}")
+        pos = pos.to(device=x.device, dtype=torch.int64)
+    if validate and pos.numel():
+        for a, ((lo, hi), (cos, _)) in enumerate(zip(ops.pos_range(pos), tabs)):
             if lo < 0 or hi >= cos.shape[0]:
                 raise IndexError(f"positions of axis {a} span [{lo}, {hi}] but its table has {cos.shape[0]} rows")
-        positions = on_gpu
-    pos = positions.to(device=x.device, dtype=torch.int64).contiguous()
+    if not pos.is_contiguous():
+        pos = pos.contiguous()
     if x.requires_grad and torch.is_grad_enabled():
         return _RotateAxes.apply(x, pos, tabs)
     return ops.rope_axes(x, pos, tabs)

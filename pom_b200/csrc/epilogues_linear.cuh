@@ -7,9 +7,59 @@
 // which the tensor cores need anyway.
 #pragma once
 #include "epilogues.cuh"
+#include "f32x2.cuh"
 #include "linear_math.cuh"
 
 namespace pomk {
+
+// 32 values of a row: v becomes act(v), and with SLOPE ps the packed act'(v).
+template <int ACT, bool SLOPE>
+__device__ __forceinline__ void linear_act32(float (&v)[32], uint32_t (&ps)[16]) {
+#pragma unroll
+  for (int i = 0; i < 32; i += 2) {
+    float s0, s1;
+    v[i] = linear_act<SLOPE, true>(ACT, v[i], s0);
+    v[i + 1] = linear_act<SLOPE, true>(ACT, v[i + 1], s1);
+    if (SLOPE) ps[i / 2] = pack_bf16x2(s0, s1);
+  }
+}
+
+// gelu of 32 values in packed pairs: the arithmetic of linear_act<SLOPE, true>.
+template <bool SLOPE>
+__device__ __forceinline__ void gelu32(float (&v)[32], uint32_t (&ps)[16]) {
+#pragma unroll
+  for (int i = 0; i < 32; i += 2) {
+    const F2 z(v[i], v[i + 1]);
+    const F2 d = fma2(F2(fabsf(z.v.x), fabsf(z.v.y)), F2(0.2316418882f), F2(1.f));
+    const F2 t(fast_rcp(d.v.x), fast_rcp(d.v.y));
+    const F2 w = mul2(mul2(z, F2(-0.72134752044f)), z);
+    const F2 e(fast_exp2(w.v.x), fast_exp2(w.v.y));
+    F2 q = fma2(F2(0.5307027145f), t, F2(-0.7265760135f));
+    q = fma2(q, t, F2(0.7107068705f));
+    q = fma2(q, t, F2(-0.142248368f));
+    q = fma2(q, t, F2(0.127414796f));
+    q = mul2(q, mul2(t, e));
+    const F2 up = fma2(q, F2(-1.f), F2(1.f));
+    const F2 phi(z.v.x < 0.f ? q.v.x : up.v.x, z.v.y < 0.f ? q.v.y : up.v.y);
+    if (SLOPE) {
+      const F2 s = fma2(mul2(z, F2(0.3989422804014327f)), e, phi);
+      ps[i / 2] = pack_bf16x2(s.v.x, s.v.y);
+    }
+    const F2 y = mul2(z, phi);
+    v[i] = y.v.x, v[i + 1] = y.v.y;
+  }
+}
+
+template <bool SLOPE>
+__device__ __forceinline__ void linear_act32(int act, float (&v)[32], uint32_t (&ps)[16]) {
+  switch (act) {
+    case POM_ACT_GELU: gelu32<SLOPE>(v, ps); break;
+    case POM_ACT_GELU_TANH: linear_act32<POM_ACT_GELU_TANH, SLOPE>(v, ps); break;
+    case POM_ACT_SILU: linear_act32<POM_ACT_SILU, SLOPE>(v, ps); break;
+    case POM_ACT_RELU: linear_act32<POM_ACT_RELU, SLOPE>(v, ps); break;
+    default: linear_act32<POM_ACT_NONE, SLOPE>(v, ps); break;
+  }
+}
 
 template <bool RES>
 struct EpiLinear {
@@ -80,19 +130,10 @@ struct EpiLinear {
         v[i] += b.x, v[i + 1] += b.y, v[i + 2] += b.z, v[i + 3] += b.w;
       }
       if (p.save_slope) {
-        uint32_t ps[16];
-#pragma unroll
-        for (int i = 0; i < 32; i += 2) {
-          float s0, s1;
-          v[i] = linear_act<true>(p.act, v[i], s0);
-          v[i + 1] = linear_act<true>(p.act, v[i + 1], s1);
-          ps[i / 2] = pack_bf16x2(s0, s1);
-        }
-        if (t.rows_valid > 0) store_block<1>(RES ? base + 4096 : base, &maps.out0, ps, lane, col, y, t.b);
+        linear_act32<true>(p.act, v, pk);
+        if (t.rows_valid > 0) store_block<1>(RES ? base + 4096 : base, &maps.out0, pk, lane, col, y, t.b);
       } else {
-        float none;
-#pragma unroll
-        for (int i = 0; i < 32; ++i) v[i] = linear_act<false>(p.act, v[i], none);
+        linear_act32<false>(p.act, v, pk);
       }
       if constexpr (RES) {
         float r[32];

@@ -43,12 +43,12 @@ __device__ __forceinline__ void few_finish(const FewDev& a, int row, int n, floa
   float v[1];
   if (a.slope) {
     float s[1];
-    v[0] = linear_act<true>(a.act, z, s[0]);
+    v[0] = linear_act<true, Piece<T, 1>::kBf16>(a.act, z, s[0]);
     p.set(s);
     p.st(static_cast<T*>(a.slope) + row * a.ld_slope + n);
   } else {
     float none;
-    v[0] = linear_act<false>(a.act, z, none);
+    v[0] = linear_act<false, Piece<T, 1>::kBf16>(a.act, z, none);
   }
   if (a.residual) {
     p.ld(static_cast<const T*>(a.residual) + row * a.ldr + n);
@@ -202,7 +202,7 @@ __global__ void __launch_bounds__(256) linear_epilogue_kernel(const FewDev a, co
     p.raw = *reinterpret_cast<const typename Piece<T, VEC>::R*>(z + r * ldz + c);  // may alias y: no read-only path
     float v[VEC], s[VEC];
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) v[e] = linear_act<true>(a.act, p.get(e) + few_bias(a, c + e), s[e]);
+    for (int e = 0; e < VEC; ++e) v[e] = linear_act<true, Piece<T, 1>::kBf16>(a.act, p.get(e) + few_bias(a, c + e), s[e]);
     if (a.slope) {
       q.set(s);
       q.st(static_cast<T*>(a.slope) + r * a.ld_slope + c);
@@ -337,9 +337,11 @@ int launch_few_f32(const FewDev& d, cudaStream_t st) {
   return launched(launch_pdl(linear_few_f32_kernel<MR>, dim3(static_cast<unsigned>(ceil_div(d.N, 8))), dim3(32 * kFewWarps), 0, st, d));
 }
 
-// Row chunks of linear_dz_kernel: about eight blocks per SM, at least 32 rows each.
-int dz_chunk(int64_t M, int64_t N, int vec) {
-  const int64_t cols = ceil_div(N, 32 * vec), want = ceil_div(8ll * sm_count(), cols);
+// Row chunks of linear_dz_kernel, at least 32 rows each.  Sums alone: one wave of three blocks per SM (32768 x 1152: 18 us;
+// eight blocks per SM: 22).  With dz to write: eight blocks per SM (32768 x 4608: 132 us, the rate of a copy; three: 138).
+int dz_chunk(int64_t M, int64_t N, int vec, bool sums_only) {
+  const int64_t cols = ceil_div(N, 32 * vec), blocks = (sums_only ? 3ll : 8ll) * sm_count();
+  const int64_t want = blocks / cols > 0 ? blocks / cols : 1;
   int64_t rows = ceil_div(ceil_div(M, want), 32) * 32;
   if (ceil_div(M, rows) > 65535) rows = ceil_div(ceil_div(M, 65535), 32) * 32;
   return static_cast<int>(rows);
@@ -354,7 +356,7 @@ BwdPlan bwd_plan(const pom_linear_args* a) {
   BwdPlan p{};
   const int per = a->dtype == POM_BF16 ? 8 : 4;
   p.vec = a->N % per || a->ld_dy % per || !aligned16(a->dy) ? 1 : per;
-  p.chunk = dz_chunk(a->M, a->N, p.vec);
+  p.chunk = dz_chunk(a->M, a->N, p.vec, !a->slope);
   p.chunks = static_cast<int>(ceil_div(a->M, p.chunk));
   p.slabs = a->dtype == POM_BF16 && a->dw ? gemm_bf16_slabs(a->N, a->K, a->M, true, true) : 1;
   auto up = [](uint64_t v) { return (v + 255) / 256 * 256; };

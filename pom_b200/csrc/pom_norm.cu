@@ -9,6 +9,7 @@
 // in registers, over the warps of a block in a fixed order, and written as one row per block; a second kernel adds
 // those rows in a fixed order: the same bits on every run.
 #include <initializer_list>
+#include "f32x2.cuh"
 #include "rows.cuh"
 
 using namespace pomk;
@@ -161,9 +162,170 @@ __global__ void __launch_bounds__(512) norm_fwd_wide_kernel(const NormDev a) {
   }
 }
 
-template <class T, class W, int VEC, int NV, int TPR>
-__global__ void __launch_bounds__(TPR == 32 ? 384 : TPR) norm_bwd_kernel(const NormDev a) {
-  extern __shared__ float scratch[];  // TPR == 32 with partial sums: 2 * D floats
+// The row's pieces a thread will read come through shared memory, kStages - 1 rows ahead, with asynchronous copies: every
+// thread copies exactly the 16 bytes that it reads itself, so no barrier stands between copy and use.
+__device__ __forceinline__ void copy16(uint4* dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copy_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+// rows in flight per thread group: what fits beside the widest rows' scale (512 threads: 196 KB at two)
+template <int TPR>
+constexpr int kBwdStages = TPR == 512 ? 2 : 3;
+
+// 16-byte pieces (VEC 8 or 4).  scratch: [w: (NV, TPR, VEC) floats][ring: stage, x or dy, piece, thread]; after the rows,
+// with TPR == 32, the first 2 * D floats hold the block's sums.
+template <class T, class W, int NV, int TPR>
+__global__ void __launch_bounds__(TPR == 32 ? 384 : TPR, TPR == 128 ? 3 : 1) norm_bwd_kernel(const NormDev a) {
+  constexpr int VEC = 16 / static_cast<int>(sizeof(T)), P2 = VEC / 2, kStages = kBwdStages<TPR>;
+  extern __shared__ uint4 scratch[];
+  __shared__ float2 sm[2 * (TPR / 32)];
+  const int t = TPR == 32 ? threadIdx.x & 31 : threadIdx.x;
+  const int sub = TPR == 32 ? threadIdx.x >> 5 : 0;
+  const int rows = TPR == 32 ? blockDim.x >> 5 : 1;
+  float* wsm = reinterpret_cast<float*>(scratch);  // piece i of thread t at (i * TPR + t) * VEC: column order
+  uint4* ring = scratch + NV * TPR * VEC / 4 + threadIdx.x;
+  const int T0 = blockDim.x;
+  griddep_wait();
+  griddep_launch();
+  const float inv_d = 1.f / static_cast<float>(a.D);
+  const bool affine = a.w != nullptr;
+  for (int c = threadIdx.x; c < NV * TPR * VEC; c += T0) {
+    Piece<W, 1> p;
+    p.zero();
+    if (affine && c < a.D) p.ld(static_cast<const W*>(a.w) + c);
+    wsm[c] = affine ? p.get(0) : 1.f;
+  }
+  const long long step = static_cast<long long>(gridDim.x) * rows;
+  const long long first = static_cast<long long>(blockIdx.x) * rows + sub;
+  auto fetch = [&](long long row, int stage) {
+    if (row < a.M) {
+      const T* x = static_cast<const T*>(a.x) + row * a.ldx;
+      const T* g = static_cast<const T*>(a.dy) + row * a.ld_dy;
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        const int c = (i * TPR + t) * VEC;
+        if (c < a.D) {
+          copy16(ring + ((stage * 2 + 0) * NV + i) * T0, x + c);
+          copy16(ring + ((stage * 2 + 1) * NV + i) * T0, g + c);
+        }
+      }
+    }
+    copy_commit();
+  };
+  for (int s = 0; s < kStages - 1; ++s) fetch(first + s * step, s);
+  float2 st = first < a.M ? __ldg(a.stats + first) : make_float2(0.f, 0.f);
+  F2 dw[NV][P2], db[NV][P2];
+#pragma unroll
+  for (int i = 0; i < NV; ++i)
+#pragma unroll
+    for (int e = 0; e < P2; ++e) dw[i][e] = db[i][e] = F2(0.f);
+  __syncthreads();
+  int slot = 0, stage = 0;
+  for (long long row = first; row < a.M; row += step) {
+    int ahead = stage + kStages - 1;
+    if (ahead >= kStages) ahead -= kStages;
+    fetch(row + (kStages - 1) * step, ahead);  // into the stage that the previous row has left
+    const float mean = st.x, r = st.y;
+    if (row + step < a.M) st = __ldg(a.stats + row + step);
+    copy_wait<kStages - 1>();
+    const F2 r2(r), off(-mean * r);
+    Piece<T, VEC> px[NV], pg[NV];
+    F2 s1(0.f), s2(0.f);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = (i * TPR + t) * VEC;
+      if (c < a.D) {
+        px[i].raw = ring[((stage * 2 + 0) * NV + i) * T0];
+        pg[i].raw = ring[((stage * 2 + 1) * NV + i) * T0];
+#pragma unroll
+        for (int e = 0; e < P2; ++e) {
+          const F2 g(pg[i].get(2 * e), pg[i].get(2 * e + 1)), x(px[i].get(2 * e), px[i].get(2 * e + 1));
+          const F2 xh = fma2(x, r2, off);
+          const float2 w = *reinterpret_cast<const float2*>(wsm + c + 2 * e);
+          const F2 h = mul2(g, F2(w.x, w.y));
+          s1 = add2(s1, h);
+          s2 = fma2(h, xh, s2);
+          dw[i][e] = fma2(g, xh, dw[i][e]);
+          db[i][e] = add2(db[i][e], g);
+        }
+      }
+    }
+    if (++stage == kStages) stage = 0;
+    if (!a.dx) continue;  // the same for every thread
+    const float2 s = row_sum2<TPR>(s1.v.x + s1.v.y, s2.v.x + s2.v.y, sm, slot);
+    slot ^= 1;
+    // dx = r h - r c1 - xh (r c2)
+    const F2 c1(-r * (s.x * inv_d)), c2(-r * (s.y * inv_d));
+    T* dx = static_cast<T*>(a.dx) + row * a.ld_dx;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = (i * TPR + t) * VEC;
+      if (c < a.D) {
+        float o[VEC];
+#pragma unroll
+        for (int e = 0; e < P2; ++e) {
+          const F2 g(pg[i].get(2 * e), pg[i].get(2 * e + 1)), x(px[i].get(2 * e), px[i].get(2 * e + 1));
+          const F2 xh = fma2(x, r2, off);
+          const float2 w = *reinterpret_cast<const float2*>(wsm + c + 2 * e);
+          const F2 d = fma2(mul2(g, F2(w.x, w.y)), r2, fma2(xh, c2, c1));
+          o[2 * e] = d.v.x, o[2 * e + 1] = d.v.y;
+        }
+        px[i].set(o);
+        px[i].st(dx + c);
+      }
+    }
+  }
+  copy_wait<0>();
+  if (!a.partial) return;
+  float* out = a.partial + static_cast<long long>(blockIdx.x) * 2 * a.D;
+  if constexpr (TPR == 32) {
+    // the warps of the block add their sums one after the other, over the ring, which nobody reads any more
+    float* sums = reinterpret_cast<float*>(scratch);
+    __syncthreads();
+    for (int turn = 0; turn < rows; ++turn) {
+      if (sub == turn) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+          const int c = (i * TPR + t) * VEC;
+          if (c < a.D) {
+#pragma unroll
+            for (int e = 0; e < P2; ++e) {
+              float2* pw = reinterpret_cast<float2*>(sums + c + 2 * e);
+              float2* pb = reinterpret_cast<float2*>(sums + a.D + c + 2 * e);
+              const float2 w = turn ? *pw : make_float2(0.f, 0.f), b = turn ? *pb : make_float2(0.f, 0.f);
+              *pw = make_float2(w.x + dw[i][e].v.x, w.y + dw[i][e].v.y);
+              *pb = make_float2(b.x + db[i][e].v.x, b.y + db[i][e].v.y);
+            }
+          }
+        }
+      }
+      __syncthreads();
+    }
+    for (int c = threadIdx.x; c < 2 * a.D; c += T0) out[c] = sums[c];
+  } else {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = (i * TPR + t) * VEC;
+      if (c < a.D) {
+#pragma unroll
+        for (int e = 0; e < P2; ++e) {
+          *reinterpret_cast<float2*>(out + c + 2 * e) = dw[i][e].v;
+          *reinterpret_cast<float2*>(out + a.D + c + 2 * e) = db[i][e].v;
+        }
+      }
+    }
+  }
+}
+
+// The same without 16-byte access (odd widths and strides, unaligned addresses): one value per piece, rows as they come.
+template <class T, class W, int NV, int TPR>
+__global__ void __launch_bounds__(TPR == 32 ? 384 : TPR) norm_bwd_odd_kernel(const NormDev a) {
+  extern __shared__ float odd_sums[];  // TPR == 32 with partial sums: 2 * D floats
   __shared__ float2 sm[2 * (TPR / 32)];
   griddep_wait();
   griddep_launch();
@@ -171,46 +333,36 @@ __global__ void __launch_bounds__(TPR == 32 ? 384 : TPR) norm_bwd_kernel(const N
   const int sub = TPR == 32 ? threadIdx.x >> 5 : 0;
   const int rows = TPR == 32 ? blockDim.x >> 5 : 1;
   const float inv_d = 1.f / static_cast<float>(a.D);
-  const bool affine = a.w != nullptr;
-  float dw[NV][VEC], db[NV][VEC];
+  float w[NV], dw[NV], db[NV];
 #pragma unroll
-  for (int i = 0; i < NV; ++i)
-#pragma unroll
-    for (int e = 0; e < VEC; ++e) dw[i][e] = db[i][e] = 0.f;
+  for (int i = 0; i < NV; ++i) {
+    const int c = i * TPR + t;
+    Piece<W, 1> p;
+    if (a.w && c < a.D) p.ld(static_cast<const W*>(a.w) + c);
+    w[i] = a.w && c < a.D ? p.get(0) : 1.f;
+    dw[i] = db[i] = 0.f;
+  }
   int slot = 0;
   for (long long row = static_cast<long long>(blockIdx.x) * rows + sub; row < a.M; row += static_cast<long long>(gridDim.x) * rows) {
     const T* x = static_cast<const T*>(a.x) + row * a.ldx;
     const T* g = static_cast<const T*>(a.dy) + row * a.ld_dy;
-    Piece<T, VEC> px[NV], pg[NV];
+    Piece<T, 1> px[NV], pg[NV];
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int c = (i * TPR + t) * VEC;
+      const int c = i * TPR + t;
       if (c < a.D) px[i].ld(x + c), pg[i].ld(g + c);
       else px[i].zero(), pg[i].zero();
     }
     const float2 st = __ldg(a.stats + row);
-    const float mean = st.x, r = st.y;
+    const float r = st.y, off = -st.x * st.y;
     float s1 = 0.f, s2 = 0.f;
-    constexpr int WV = VEC * static_cast<int>(sizeof(W)) <= 16 ? VEC : 16 / static_cast<int>(sizeof(W));
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int c = (i * TPR + t) * VEC;
-      if (c < a.D) {
-#pragma unroll
-        for (int k = 0; k < VEC; k += WV) {
-          Piece<W, WV> pw;
-          if (affine) pw.ld(static_cast<const W*>(a.w) + c + k);
-#pragma unroll
-          for (int e = 0; e < WV; ++e) {
-            const float gv = pg[i].get(k + e), xh = (px[i].get(k + e) - mean) * r;
-            const float h = affine ? gv * pw.get(e) : gv;
-            s1 += h;
-            s2 = fmaf(h, xh, s2);
-            dw[i][k + e] = fmaf(gv, xh, dw[i][k + e]);
-            db[i][k + e] += gv;
-          }
-        }
-      }
+      const float gv = pg[i].get(0), xh = fmaf(px[i].get(0), r, off), h = gv * w[i];  // gv is 0 behind the row's end
+      s1 += h;
+      s2 = fmaf(h, xh, s2);
+      dw[i] = fmaf(gv, xh, dw[i]);
+      db[i] += gv;
     }
     if (!a.dx) continue;  // the same for every thread
     const float2 s = row_sum2<TPR>(s1, s2, sm, slot);
@@ -219,20 +371,9 @@ __global__ void __launch_bounds__(TPR == 32 ? 384 : TPR) norm_bwd_kernel(const N
     T* dx = static_cast<T*>(a.dx) + row * a.ld_dx;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int c = (i * TPR + t) * VEC;
+      const int c = i * TPR + t;
       if (c < a.D) {
-        float o[VEC];
-#pragma unroll
-        for (int k = 0; k < VEC; k += WV) {
-          Piece<W, WV> pw;
-          if (affine) pw.ld(static_cast<const W*>(a.w) + c + k);
-#pragma unroll
-          for (int e = 0; e < WV; ++e) {
-            const float gv = pg[i].get(k + e), xh = (px[i].get(k + e) - mean) * r;
-            const float h = affine ? gv * pw.get(e) : gv;
-            o[k + e] = r * (h - c1 - xh * c2);
-          }
-        }
+        const float o[1] = {r * (pg[i].get(0) * w[i] - c1 - fmaf(px[i].get(0), r, off) * c2)};
         px[i].set(o);
         px[i].st(dx + c);
       }
@@ -241,32 +382,25 @@ __global__ void __launch_bounds__(TPR == 32 ? 384 : TPR) norm_bwd_kernel(const N
   if (!a.partial) return;
   float* out = a.partial + static_cast<long long>(blockIdx.x) * 2 * a.D;
   if constexpr (TPR == 32) {
-    // the warps of the block add their sums one after the other
     for (int turn = 0; turn < rows; ++turn) {
       if (sub == turn) {
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-          const int c = (i * TPR + t) * VEC;
+          const int c = i * TPR + t;
           if (c < a.D) {
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) {
-              scratch[c + e] = (turn ? scratch[c + e] : 0.f) + dw[i][e];
-              scratch[a.D + c + e] = (turn ? scratch[a.D + c + e] : 0.f) + db[i][e];
-            }
+            odd_sums[c] = (turn ? odd_sums[c] : 0.f) + dw[i];
+            odd_sums[a.D + c] = (turn ? odd_sums[a.D + c] : 0.f) + db[i];
           }
         }
       }
       __syncthreads();
     }
-    for (int c = threadIdx.x; c < 2 * a.D; c += blockDim.x) out[c] = scratch[c];
+    for (int c = threadIdx.x; c < 2 * a.D; c += blockDim.x) out[c] = odd_sums[c];
   } else {
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int c = (i * TPR + t) * VEC;
-      if (c < a.D) {
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) out[c + e] = dw[i][e], out[a.D + c + e] = db[i][e];
-      }
+      const int c = i * TPR + t;
+      if (c < a.D) out[c] = dw[i], out[a.D + c] = db[i];
     }
   }
 }
@@ -343,6 +477,7 @@ NormPlan norm_plan(int D, int dtype, bool wide_access) {
   return NormPlan{1, 0, 0};
 }
 
+constexpr int kMaxBwdSmem = 200 * 1024;
 constexpr int kFwdWarps = 8, kBwdWarps = 12, kWideSplits = 64;
 
 int bwd_blocks(int64_t M, const NormPlan& p) {
@@ -356,8 +491,25 @@ int launch_norm(const NormDev& d, bool bwd, int blocks, cudaStream_t st) {
   cudaError_t e;
   if (bwd) {
     const int threads = TPR == 32 ? 32 * kBwdWarps : TPR;
-    const size_t smem = TPR == 32 && d.partial ? 2 * static_cast<size_t>(d.D) * sizeof(float) : 0;
-    e = launch_pdl(norm_bwd_kernel<T, W, VEC, NV, TPR>, dim3(blocks), dim3(threads), smem, st, d);
+    const size_t sums = TPR == 32 && d.partial ? 2 * static_cast<size_t>(d.D) * sizeof(float) : 0;
+    if constexpr (VEC > 1) {
+      const int ring = NV * TPR * VEC * 4 + kBwdStages<TPR> * 2 * NV * threads * 16;
+      const int smem = static_cast<int>(sums) > ring ? static_cast<int>(sums) : ring;
+      static_assert(NV * TPR * VEC * 4 + kBwdStages<TPR> * 2 * NV * (TPR == 32 ? 32 * kBwdWarps : TPR) * 16 <= kMaxBwdSmem);
+      static std::atomic<uint64_t> attr_set{0};
+      auto kern = norm_bwd_kernel<T, W, NV, TPR>;
+      const int rc = once_per_device(attr_set, [&] {
+        if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxBwdSmem) != cudaSuccess) {
+          (void)cudaGetLastError();
+          return static_cast<int>(POM_ERR_CUDA);
+        }
+        return static_cast<int>(POM_OK);
+      });
+      if (rc) return rc;
+      e = launch_pdl(kern, dim3(blocks), dim3(threads), smem, st, d);
+    } else {
+      e = launch_pdl(norm_bwd_odd_kernel<T, W, NV, TPR>, dim3(blocks), dim3(threads), sums, st, d);
+    }
   } else {
     const int threads = TPR == 32 ? 32 * kFwdWarps : TPR;
     const int64_t want = ceil_div(d.M, TPR == 32 ? kFwdWarps : 1), cap = 32ll * sm_count();

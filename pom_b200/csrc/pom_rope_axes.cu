@@ -6,8 +6,9 @@
 //     y[k] = x[k] cos - x[k + s] sin        y[k + s] = x[k] sin + x[k + s] cos
 // The transpose (the backward pass) turns the other way.  Channels behind the last section are copied.
 //
-// A thread owns VEC pairs (16 bytes on either side of the pairing where alignment allows) of one token and walks the
-// heads, so that its cosines and sines are read once for all of them.
+// A thread owns VEC pairs (16 bytes on either side of the pairing where alignment allows) of one head and walks a run of
+// tokens, two at a time: where its channels lie is found once, and a step of the walk is two loads of x, one position and
+// the table row that it names.
 #include <limits.h>
 #include <initializer_list>
 #include "rows.cuh"
@@ -18,6 +19,7 @@ using namespace pomh;
 namespace {
 
 constexpr int kMaxAxes = POM_ROPE_MAX_AXES;
+constexpr int kThreads = 256, kPerSm = 8, kRun = 8;
 
 struct AxesDev {
   const void* x;
@@ -28,44 +30,66 @@ struct AxesDev {
   int len[kMaxAxes], pairs[kMaxAxes];
   long long xs_b, xs_n, xs_h;  // strides of x; y is contiguous
   long long B, N;
-  int H, D, axes, units, pair_units;
+  int H, D, axes, units, pair_units, run;
   int pos_per_sample;
   float sign;
 };
 
 template <class T, int VEC>
-__global__ void __launch_bounds__(256) rope_axes_kernel(const AxesDev a) {
+__global__ void __launch_bounds__(kThreads) rope_axes_kernel(const AxesDev a) {
   griddep_wait();
   griddep_launch();
-  const long long total = a.B * a.N * a.units;
-  for (long long i = blockIdx.x * 256ll + threadIdx.x; i < total; i += gridDim.x * 256ll) {
-    const long long tok = i / a.units;
-    int u = static_cast<int>(i - tok * a.units);
-    const long long b = tok / a.N, n = tok - b * a.N;
-    const T* x = static_cast<const T*>(a.x) + b * a.xs_b + n * a.xs_n;
-    T* y = static_cast<T*>(a.y) + tok * a.H * a.D;
-    if (u >= a.pair_units) {  // a copied channel block
-      const int c = a.D - (a.units - u) * VEC;
-      for (int h = 0; h < a.H; ++h) {
-        Piece<T, VEC> p;
-        p.ld(x + h * a.xs_h + c);
-        p.st(y + static_cast<long long>(h) * a.D + c);
-      }
+  const int hu = blockIdx.y * blockDim.x + threadIdx.x;
+  if (hu >= a.H * a.units) return;
+  const int h = hu / a.units;
+  int u = hu - h * a.units;
+  // where this thread's channels lie: section `axis`, pairs k .. k + VEC of it, first channel lo + k; axis < 0: copied
+  int axis = -1, lo = 0, s = 0, k = a.D - (a.units - u) * VEC;
+  const float *ct = nullptr, *st = nullptr;
+  int len = 0;
+  if (u < a.pair_units) {
+    axis = 0;
+    while (u * VEC >= a.pairs[axis]) u -= a.pairs[axis] / VEC, lo += 2 * a.pairs[axis], ++axis;
+    s = a.pairs[axis], k = u * VEC, len = a.len[axis];
+    ct = a.cos[axis] + k, st = a.sin[axis] + k;
+  }
+  const T* __restrict__ x = static_cast<const T*>(a.x) + h * a.xs_h + lo + k;
+  T* __restrict__ y = static_cast<T*>(a.y) + h * static_cast<long long>(a.D) + lo + k;
+  const long long* __restrict__ pos = a.pos + axis;
+  const long long y_tok = static_cast<long long>(a.H) * a.D, total = a.B * a.N;
+  const long long tok0 = static_cast<long long>(blockIdx.x) * a.run * blockDim.y + threadIdx.y;
+  const long long stop = tok0 - threadIdx.y + static_cast<long long>(a.run) * blockDim.y, end = stop < total ? stop : total;
+  // what a token needs from global memory, one token ahead of its turn
+  Piece<T, VEC> n1, n2;
+  long long np = 0;
+  auto fetch = [&](long long tok) {
+    if (tok >= end) return;
+    const long long b = total <= 0x7fffffff ? static_cast<unsigned>(tok) / static_cast<unsigned>(a.N) : tok / a.N;
+    const long long n = tok - b * a.N;
+    const T* xr = x + b * a.xs_b + n * a.xs_n;
+    n1.ld(xr);
+    if (axis >= 0) {
+      n2.ld(xr + s);
+      np = __ldg(pos + (a.pos_per_sample ? tok : n) * a.axes);
+    }
+  };
+  fetch(tok0);
+  for (long long tok = tok0; tok < end; tok += blockDim.y) {
+    Piece<T, VEC> p1 = n1, p2 = n2;
+    const long long p = np;
+    fetch(tok + blockDim.y);
+    T* yr = y + tok * y_tok;
+    if (axis < 0) {
+      p1.st(yr);
       continue;
     }
-    int axis = 0, lo = 0;  // section and its first channel
-    while (u * VEC >= a.pairs[axis]) u -= a.pairs[axis] / VEC, lo += 2 * a.pairs[axis], ++axis;
-    const int s = a.pairs[axis], k = u * VEC;
-    const long long p = __ldg(a.pos + (a.pos_per_sample ? tok : n) * a.axes + axis);
     float cs[VEC], sn[VEC];
-    if (p >= 0 && p < a.len[axis]) {
-      const float* ct = a.cos[axis] + p * s + k;
-      const float* st = a.sin[axis] + p * s + k;
+    if (p >= 0 && p < len) {
       constexpr int F = VEC < 4 ? VEC : 4;
 #pragma unroll
       for (int e = 0; e < VEC; e += F) {
         Piece<float, F> pc, ps;
-        pc.ld(ct + e), ps.ld(st + e);
+        pc.ld(ct + p * s + e), ps.ld(st + p * s + e);
 #pragma unroll
         for (int f = 0; f < F; ++f) cs[e + f] = pc.get(f), sn[e + f] = a.sign * ps.get(f);
       }
@@ -73,21 +97,16 @@ __global__ void __launch_bounds__(256) rope_axes_kernel(const AxesDev a) {
 #pragma unroll
       for (int e = 0; e < VEC; ++e) cs[e] = sn[e] = __int_as_float(0x7fc00000);
     }
-    for (int h = 0; h < a.H; ++h) {
-      Piece<T, VEC> p1, p2;
-      p1.ld(x + h * a.xs_h + lo + k);
-      p2.ld(x + h * a.xs_h + lo + s + k);
-      float v1[VEC], v2[VEC];
+    float v1[VEC], v2[VEC];
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) {
-        const float x1 = p1.get(e), x2 = p2.get(e);
-        v1[e] = x1 * cs[e] - x2 * sn[e];
-        v2[e] = x1 * sn[e] + x2 * cs[e];
-      }
-      p1.set(v1), p2.set(v2);
-      p1.st(y + static_cast<long long>(h) * a.D + lo + k);
-      p2.st(y + static_cast<long long>(h) * a.D + lo + s + k);
+    for (int e = 0; e < VEC; ++e) {
+      const float x1 = p1.get(e), x2 = p2.get(e);
+      v1[e] = x1 * cs[e] - x2 * sn[e];
+      v2[e] = x1 * sn[e] + x2 * cs[e];
     }
+    p1.set(v1), p2.set(v2);
+    p1.st(yr);
+    p2.st(yr + s);
   }
 }
 
@@ -121,9 +140,9 @@ __global__ void __launch_bounds__(1024) pos_range_kernel(const long long* __rest
   }
 }
 
-// Pairs per thread: 16 bytes of x where every section, stride and address allows it, else 4 bytes, else one value.
+// Pairs per thread: 16 bytes of x where every section, stride and address allows it, else 8, 4 bytes, else one value.
 int axes_vec(const pom_rope_axes_args* a, int wide) {
-  for (int v : {wide, 2}) {
+  for (int v : {wide, 4, 2}) {
     bool ok = a->D % v == 0 && a->xs_b % v == 0 && a->xs_n % v == 0 && a->xs_h % v == 0;
     const uintptr_t xm = static_cast<uintptr_t>(v) * (a->dtype == POM_BF16 ? 2 : 4) - 1;
     const uintptr_t fm = (v < 4 ? v : 4) * 4 - 1;
@@ -164,13 +183,22 @@ int pom_rope_axes(const pom_rope_axes_args* a, void* stream) {
   d.units = d.pair_units + static_cast<int>((a->D - 2 * total_pairs) / vec);
   d.pos_per_sample = a->pos_per_sample;
   d.sign = a->transpose ? -1.f : 1.f;
-  const int64_t want = ceil_div(a->B * a->N * d.units, 256), cap = 64ll * sm_count();
-  const dim3 grid(static_cast<unsigned>(want < cap ? want : cap));
+  // blockDim = (pieces of a token: heads x units, tokens); blockIdx = (token lanes, pieces)
+  const int64_t per_tok = static_cast<int64_t>(a->H) * d.units, tokens = a->B * a->N;
+  if (per_tok > 65535ll * 256) return POM_ERR_TOO_LARGE;
+  const int64_t bx = per_tok < 256 ? per_tok : 256, by = kThreads / bx, pieces = ceil_div(per_tok, bx);
+  int64_t run = tokens * pieces / (kPerSm * sm_count() * by);
+  run = run < 1 ? 1 : run > kRun ? kRun : run;
+  if (ceil_div(tokens, run * by) > INT32_MAX) return POM_ERR_TOO_LARGE;
+  d.run = static_cast<int>(run);
+  const dim3 grid(static_cast<unsigned>(ceil_div(tokens, run * by)), static_cast<unsigned>(pieces));
+  const dim3 block(static_cast<unsigned>(bx), static_cast<unsigned>(by));
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   cudaError_t e;
-#define POM_AXES(T, V) e = launch_pdl(rope_axes_kernel<T, V>, grid, dim3(256), 0, st, d)
+#define POM_AXES(T, V) e = launch_pdl(rope_axes_kernel<T, V>, grid, block, 0, st, d)
   if (a->dtype == POM_BF16) {
     if (vec == 8) POM_AXES(__nv_bfloat16, 8);
+    else if (vec == 4) POM_AXES(__nv_bfloat16, 4);
     else if (vec == 2) POM_AXES(__nv_bfloat16, 2);
     else POM_AXES(__nv_bfloat16, 1);
   } else {

@@ -959,22 +959,39 @@ def rows_of(t: torch.Tensor, align: bool = False):
     return t, ld
 
 
+def _same_device(x: torch.Tensor, *others) -> None:
+    """All tensors on x's GPU (others may be None)."""
+    i = x.get_device()
+    if i < 0:
+        raise RuntimeError("pom_b200 runs on CUDA tensors only (no CPU fallback)")
+    for t in others:
+        if t is not None and t.get_device() != i:
+            if t.get_device() < 0:
+                raise RuntimeError("pom_b200 runs on CUDA tensors only (no CPU fallback)")
+            raise RuntimeError("all tensors of one call must live on the same GPU")
+
+
+_DTYPE = {torch.bfloat16: _abi.POM_BF16, torch.float32: _abi.POM_F32}
+
+
 def layer_norm_fwd(x: torch.Tensor, weight: Optional[torch.Tensor], bias: Optional[torch.Tensor], eps: float,
                    want_stats: bool):
     """Layer norm over the last dimension: (y, stats), stats (M, 2) fp32 = mean and 1 / sqrt(var + eps) of every row, or
     None.  ``weight`` and ``bias`` contiguous, of one dtype."""
-    dev = _require_cuda(x, weight, bias)
+    _same_device(x, weight, bias)
     x, ld = rows_of(x)
     D = x.shape[-1]
     M = x.numel() // D
-    y = torch.empty(x.shape, dtype=x.dtype, device=dev)
-    stats = torch.empty((M, 2), dtype=torch.float32, device=dev) if want_stats else None
+    y = torch.empty_like(x, memory_format=torch.contiguous_format)
+    stats = x.new_empty((M, 2), dtype=torch.float32) if want_stats else None
     if M:
         a = LayerNormArgs()
         a.x, a.y, a.M, a.ldx, a.ldy, a.D, a.eps = x.data_ptr(), y.data_ptr(), M, ld, D, D, eps
-        a.dtype = a.wdtype = _abi.dtype_code(x.dtype)
+        a.dtype = a.wdtype = _DTYPE[x.dtype]
         if weight is not None:
-            a.weight, a.bias, a.wdtype = weight.data_ptr(), ptr(bias), _abi.dtype_code(weight.dtype)
+            a.weight, a.wdtype = weight.data_ptr(), _DTYPE[weight.dtype]
+            if bias is not None:
+                a.bias = bias.data_ptr()
         if stats is not None:
             a.stats = stats.data_ptr()
         _abi.check(_abi.lib().pom_layer_norm_fwd(C.byref(a), _abi.stream_ptr()), "pom_layer_norm_fwd")
@@ -984,36 +1001,40 @@ def layer_norm_fwd(x: torch.Tensor, weight: Optional[torch.Tensor], bias: Option
 def layer_norm_bwd(dy: torch.Tensor, x: torch.Tensor, weight: Optional[torch.Tensor], stats: torch.Tensor, *,
                    want_dx: bool, want_dw: bool, want_db: bool):
     """(dx, dweight, dbias) of :func:`layer_norm_fwd`; what is not wanted is None."""
-    dev = _require_cuda(dy, x, weight, stats)
+    _same_device(dy, x, weight, stats)
     x, ldx = rows_of(x)
     dy, ldg = rows_of(dy)
     D = x.shape[-1]
     M = x.numel() // D
-    dx = torch.empty(x.shape, dtype=x.dtype, device=dev) if want_dx else None
+    dx = torch.empty_like(x, memory_format=torch.contiguous_format) if want_dx else None
     dw = torch.empty_like(weight) if want_dw else None
     db = torch.empty_like(weight) if want_db else None
     if M == 0:
         return dx, dw if dw is None else fill_zero(dw), db if db is None else fill_zero(db)
     a = LayerNormArgs()
-    a.x, a.dy, a.stats, a.weight = x.data_ptr(), dy.data_ptr(), stats.data_ptr(), ptr(weight)
-    a.dx, a.dweight, a.dbias = ptr(dx), ptr(dw), ptr(db)
+    a.x, a.dy, a.stats = x.data_ptr(), dy.data_ptr(), stats.data_ptr()
     a.M, a.ldx, a.ld_dy, a.ld_dx, a.D = M, ldx, ldg, D, D
-    a.dtype = _abi.dtype_code(x.dtype)
-    a.wdtype = a.dtype if weight is None else _abi.dtype_code(weight.dtype)
+    a.dtype = a.wdtype = _DTYPE[x.dtype]
+    if dx is not None:
+        a.dx = dx.data_ptr()
     L = _abi.lib()
-    if want_dw or want_db:
-        ws = torch.empty((int(L.pom_layer_norm_bwd_workspace(C.byref(a))),), dtype=torch.uint8, device=dev)
-        a.workspace = ws.data_ptr()
+    if weight is not None:
+        a.weight, a.wdtype = weight.data_ptr(), _DTYPE[weight.dtype]
+        if dw is not None:
+            a.dweight = dw.data_ptr()
+        if db is not None:
+            a.dbias = db.data_ptr()
+        if dw is not None or db is not None:
+            ws = stats.new_empty(L.pom_layer_norm_bwd_workspace(C.byref(a)) // 4)
+            a.workspace = ws.data_ptr()
     _abi.check(L.pom_layer_norm_bwd(C.byref(a), _abi.stream_ptr()), "pom_layer_norm_bwd")
     return dx, dw, db
 
 
-def _linear_args(x, w, bias, act, M, N, K, ldx, ldw) -> LinearArgs:
+def _linear_args(x, w, act, M, N, K, ldx, ldw) -> LinearArgs:
     a = LinearArgs()
     a.x, a.w, a.M, a.N, a.K, a.ldx, a.ldw = x.data_ptr(), w.data_ptr(), M, N, K, ldx, ldw
-    a.act, a.dtype = _abi.ACTIVATIONS[act], _abi.dtype_code(x.dtype)
-    if bias is not None:
-        a.bias, a.bias_dtype = bias.data_ptr(), _abi.dtype_code(bias.dtype)
+    a.act, a.dtype = _abi.ACTIVATIONS[act], _DTYPE[x.dtype]
     return a
 
 
@@ -1021,18 +1042,20 @@ def linear_fwd(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor], a
                residual: Optional[torch.Tensor], want_slope: bool):
     """act(x·wᵀ + bias) + residual: (y, slope), slope (M, N) = act'(x·wᵀ + bias) or None.  x (..., K), w (N, K), both bf16
     (K and N multiples of 8) or both float32; ``bias`` contiguous, bf16 or float32."""
-    dev = _require_cuda(x, w, bias, residual)
+    _same_device(x, w, bias, residual)
     bf16 = x.dtype == torch.bfloat16
     x, ldx = rows_of(x, bf16)
     w, ldw = rows_of(w, bf16)
     N, K = w.shape
     M = x.numel() // K
-    y = torch.empty((*x.shape[:-1], N), dtype=x.dtype, device=dev)
-    slope = torch.empty((M, N), dtype=x.dtype, device=dev) if want_slope else None
+    y = x.new_empty((*x.shape[:-1], N))
+    slope = x.new_empty((M, N)) if want_slope else None
     if M == 0:
         return y, slope
-    a = _linear_args(x, w, bias, act, M, N, K, ldx, ldw)
+    a = _linear_args(x, w, act, M, N, K, ldx, ldw)
     a.y, a.ldy = y.data_ptr(), N
+    if bias is not None:
+        a.bias, a.bias_dtype = bias.data_ptr(), _DTYPE[bias.dtype]
     if slope is not None:
         a.slope = slope.data_ptr()
     if residual is not None:
@@ -1040,52 +1063,56 @@ def linear_fwd(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor], a
         a.residual = residual.data_ptr()
     L = _abi.lib()
     if bf16 or L.pom_linear_few_rows(C.byref(a)):
-        _abi.check(L.pom_linear_fwd(C.byref(a), _abi.status_word(dev).data_ptr(), _abi.stream_ptr()), "pom_linear_fwd")
+        _abi.check(L.pom_linear_fwd(C.byref(a), _abi.status_word(x.device).data_ptr(), _abi.stream_ptr()), "pom_linear_fwd")
         return y, slope
-    y2 = y.view(M, N)
-    gemm(x.as_strided((M, K), (ldx, 1)), w.as_strided((N, K), (ldw, 1)), out=y2)
+    gemm(x.as_strided((M, K), (ldx, 1)), w.as_strided((N, K), (ldw, 1)), out=y.view(M, N))
     if bias is not None or residual is not None or act is not None:
-        _abi.check(L.pom_linear_epilogue(C.byref(a), y.data_ptr(), N, _abi.stream_ptr()), "pom_linear_epilogue")
+        _abi.check(L.pom_linear_epilogue(C.byref(a), a.y, N, _abi.stream_ptr()), "pom_linear_epilogue")
     return y, slope
 
 
 def linear_bwd(dy: torch.Tensor, x: torch.Tensor, w: torch.Tensor, slope: Optional[torch.Tensor], *, want_dx: bool,
                want_dw: bool, bias_dtype: Optional[torch.dtype]):
     """(dx, dw, dbias) of :func:`linear_fwd` (dbias where ``bias_dtype`` is given); what is not wanted is None."""
-    dev = _require_cuda(dy, x, w, slope)
+    _same_device(dy, x, w, slope)
     bf16 = x.dtype == torch.bfloat16
     x, ldx = rows_of(x, bf16)
     w, ldw = rows_of(w, bf16)
     N, K = w.shape
     M = x.numel() // K
-    dx = torch.empty(x.shape, dtype=x.dtype, device=dev) if want_dx else None
-    dw = torch.empty((N, K), dtype=w.dtype, device=dev) if want_dw else None
-    db = torch.empty((N,), dtype=bias_dtype, device=dev) if bias_dtype is not None else None
+    dx = torch.empty_like(x, memory_format=torch.contiguous_format) if want_dx else None
+    dw = w.new_empty((N, K)) if want_dw else None
+    db = w.new_empty(N, dtype=bias_dtype) if bias_dtype is not None else None
     if M == 0:
         return dx, dw if dw is None else fill_zero(dw), db if db is None else fill_zero(db)
     dy, ldg = rows_of(dy, bf16)
-    a = _linear_args(x, w, None, None, M, N, K, ldx, ldw)
-    a.dy, a.ld_dy, a.slope, a.dbias = dy.data_ptr(), ldg, ptr(slope), ptr(db)
+    a = _linear_args(x, w, None, M, N, K, ldx, ldw)
+    a.dy, a.ld_dy = dy.data_ptr(), ldg
+    if slope is not None:
+        a.slope = slope.data_ptr()
     if db is not None:
-        a.bias_dtype = _abi.dtype_code(bias_dtype)
+        a.dbias, a.bias_dtype = db.data_ptr(), _DTYPE[bias_dtype]
     dz = None
     if bf16:
         a.dx, a.dw = ptr(dx), ptr(dw)
     elif slope is not None:
-        dz = torch.empty((M, N), dtype=x.dtype, device=dev)
+        dz = torch.empty_like(slope)
         a.dz = dz.data_ptr()
     L = _abi.lib()
-    nbytes = int(L.pom_linear_bwd_workspace(C.byref(a)))
+    nbytes = L.pom_linear_bwd_workspace(C.byref(a))
     if nbytes:
-        ws = torch.empty((nbytes,), dtype=torch.uint8, device=dev)
+        ws = x.new_empty(nbytes, dtype=torch.uint8)
         a.workspace = ws.data_ptr()
-    _abi.check(L.pom_linear_bwd(C.byref(a), _abi.status_word(dev).data_ptr(), _abi.stream_ptr()), "pom_linear_bwd")
+    _abi.check(L.pom_linear_bwd(C.byref(a), _abi.status_word(x.device).data_ptr(), _abi.stream_ptr()), "pom_linear_bwd")
     if not bf16:
         if dz is None:
             dz = dy.as_strided((M, N), (ldg, 1))
         planes = F32Planes()  # of dz, which enters both products
         if want_dw:
-            gemm(dz, x.as_strided((M, K), (ldx, 1)), a_mn=True, b_mn=True, out=dw, a_planes=planes)
+            # a sum over many rows with few output tiles: only an accumulated product is cut along its sum
+            cut = f32_planes_pay(M)
+            gemm(dz, x.as_strided((M, K), (ldx, 1)), a_mn=True, b_mn=True, out=fill_zero(dw) if cut else dw, accumulate=cut,
+                 a_planes=planes)
         if want_dx:
             gemm(dz, w.as_strided((N, K), (ldw, 1)), b_mn=True, out=dx.view(M, K), a_planes=planes)
     return dx, dw, db
@@ -1094,22 +1121,40 @@ def linear_bwd(dy: torch.Tensor, x: torch.Tensor, w: torch.Tensor, slope: Option
 def rope_axes(x: torch.Tensor, pos: torch.Tensor, tables, transpose: bool = False) -> torch.Tensor:
     """Rotation of x (B, N, D) or (B, N, H, D) by positions of several axes (``pom_rope_axes``).  pos (N, A) or (B, N, A)
     int64 contiguous; ``tables``: one (cos, sin) pair of contiguous fp32 (rows, pairs) tensors per axis."""
-    dev = _require_cuda(x, pos, *(t for cs in tables for t in cs))
-    if x.stride(-1) != 1 and x.shape[-1] > 1:
+    _same_device(x, pos)
+    stride, shape = x.stride(), x.shape
+    if stride[-1] != 1 and shape[-1] > 1:
         x = x.contiguous()
-    y = torch.empty(x.shape, dtype=x.dtype, device=dev)
+        stride = x.stride()
+    y = x.new_empty(shape)
+    a = RopeAxesArgs()
+    a.B, a.N, a.D = shape[0], shape[1], shape[-1]
     if y.numel() == 0:
         return y
-    a = RopeAxesArgs()
     a.x, a.y, a.pos = x.data_ptr(), y.data_ptr(), pos.data_ptr()
-    for i, (c, s) in enumerate(tables):
-        a.cos[i], a.sin[i], a.len[i], a.pairs[i] = c.data_ptr(), s.data_ptr(), c.shape[0], c.shape[1]
+    axes = len(tables)
+    (c, s) = tables[0]
+    a.cos0, a.sin0, (a.len0, a.pairs0) = c.data_ptr(), s.data_ptr(), c.shape
+    if axes > 1:
+        (c, s) = tables[1]
+        a.cos1, a.sin1, (a.len1, a.pairs1) = c.data_ptr(), s.data_ptr(), c.shape
+    if axes > 2:
+        (c, s) = tables[2]
+        a.cos2, a.sin2, (a.len2, a.pairs2) = c.data_ptr(), s.data_ptr(), c.shape
+    if axes > 3:
+        (c, s) = tables[3]
+        a.cos3, a.sin3, (a.len3, a.pairs3) = c.data_ptr(), s.data_ptr(), c.shape
     # a dimension of size 1 is never stepped over: its stride (PyTorch may report any) must not cost the wide access
-    st = [s if n > 1 else 0 for n, s in zip(x.shape, x.stride())]
-    a.xs_b, a.xs_n, a.xs_h = st[0], st[1], st[2] if x.dim() == 4 else 0
-    a.B, a.N, a.H, a.D = x.shape[0], x.shape[1], x.shape[2] if x.dim() == 4 else 1, x.shape[-1]
-    a.axes, a.dtype = len(tables), _abi.dtype_code(x.dtype)
-    a.pos_per_sample, a.transpose = int(pos.dim() == 3), int(transpose)
+    if shape[0] > 1:
+        a.xs_b = stride[0]
+    if shape[1] > 1:
+        a.xs_n = stride[1]
+    a.H = 1
+    if len(shape) == 4:
+        a.H = shape[2]
+        if shape[2] > 1:
+            a.xs_h = stride[2]
+    a.axes, a.dtype, a.pos_per_sample, a.transpose = axes, _DTYPE[x.dtype], pos.dim() == 3, transpose
     _abi.check(_abi.lib().pom_rope_axes(C.byref(a), _abi.stream_ptr()), "pom_rope_axes")
     return y
 

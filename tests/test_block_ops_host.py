@@ -106,9 +106,9 @@ def test_the_library_refuses_bad_arguments_before_it_launches():
     assert L.pom_rope_axes(ctypes.byref(r), None) == -4
     r.axes, r.B, r.N, r.H, r.D = 1, 1, 1, 1, 8
     assert L.pom_rope_axes(ctypes.byref(r), None) == -8
-    r.cos[0] = r.sin[0] = 16
+    r.cos0 = r.sin0 = 16
     assert L.pom_rope_axes(ctypes.byref(r), None) == -1
-    r.len[0], r.pairs[0] = 4, 5
+    r.len0, r.pairs0 = 4, 5
     assert L.pom_rope_axes(ctypes.byref(r), None) == -1  # ten channels of eight
     assert L.pom_pos_range(None, 4, 1, None, None) == -8
 
