@@ -18,6 +18,41 @@ namespace pomh {
 
 namespace {
 
+struct SlabPlan {
+  TilePlan tile;
+  int slabs;
+};
+
+// Whether a product is worth cutting along K into slabs that a second kernel adds, and how.  Estimated time in
+// microseconds: 4 for the launch and the filling of the pipeline, per wave 1 for its epilogue and, per 64 of K, what one
+// tile takes to arrive in shared memory (about 64 bytes a cycle and SM, which bounds a tile before its MMAs do; measured
+// 0.285 / 0.37 / 0.335 for 128 and 256 columns of one CTA and 256 of a pair), and for slabs 3 for the second launch and
+// their traffic at 6 TB/s.  Measured against one slab: 512 x 1152 x 4608 24.6 -> 13.7 us before the second kernel (4
+// slabs), 256 x 1024 x 4096 21.9 -> 9.2 (8); 2048 x 1024 x 4096 24.3 -> 20.8 (2), which the second kernel undoes: stays whole.
+SlabPlan pick_slabs(const Operands& o) {
+  struct Cand {
+    bool pair;
+    int bn;
+    double per_block;
+  };
+  const Cand cands[3] = {{true, 256, 0.335}, {false, 256, 0.37}, {false, 128, 0.285}};
+  const long long kb = ceil_div(o.K, kBK);
+  const double slab_us = static_cast<double>(o.M) * static_cast<double>(o.N) * 8.0 / 6e6;
+  SlabPlan best{TilePlan{true, 256}, 1};
+  double best_cost = -1.0;
+  for (const Cand& c : cands) {
+    const long long tiles = (c.pair ? pair_rows(o) : ceil_div(o.M, kBM)) * ceil_div(o.N, c.bn);
+    const int slots = c.pair ? sm_count() / 2 : sm_count();
+    for (int s = 1; s <= 16 && (s == 1 || kb / s >= 4); ++s) {
+      const long long per = ceil_div(kb, s);
+      if (ceil_div(kb, per) != s) continue;  // an empty slab
+      const double cost = ceil_div(tiles * s, slots) * (per * c.per_block + 1.0) + (s > 1 ? 3.0 + s * slab_us : 0.0);
+      if (best_cost < 0 || cost < best_cost * 0.97) best_cost = cost, best = SlabPlan{TilePlan{c.pair, c.bn}, s};
+    }
+  }
+  return best;
+}
+
 // `slabs` > 1: fp32 output, the K splits' sums side by side (M * ldc elements apart).
 int gemm_bf16_any(const pom_gemm_args* a, const float* tile_weight, int dead_k, int slabs, int* status, cudaStream_t st) {
   if (!a || !a->C) return POM_ERR_NULL;
@@ -41,7 +76,8 @@ int gemm_bf16_any(const pom_gemm_args* a, const float* tile_weight, int dead_k, 
     split = 1;
   }
   if (slabs > 1) split = slabs;
-  const TilePlan plan = pick_plan(o, true, slabs > 0 || (a->out_mode == POM_OUT_F32_ACCUM && a->split_k == 0));
+  const TilePlan plan = slabs > 1 ? pick_slabs(o).tile
+                                  : pick_plan(o, true, a->out_mode == POM_OUT_F32_ACCUM && a->split_k == 0);
   if (split == 0) split = pick_split(plan_units(o, plan), ceil_div(a->K, kBK), plan.pair ? sm_count() / 2 : sm_count());
   EpiStore::Params ep;
   ep.C = a->C;
@@ -72,10 +108,7 @@ int gemm_bf16_dead_k(const pom_gemm_args* a, const float* tile_weight, int dead_
 
 int gemm_bf16_slabs(int64_t M, int64_t N, int64_t K, bool a_mn, bool b_mn) {
   const Operands o{nullptr, nullptr, M, N, K, 0, 0, 1, a_mn, b_mn};
-  const TilePlan plan = pick_plan(o, true, true);
-  const long long kb = ceil_div(K, kBK);
-  const int split = pick_split(plan_units(o, plan), kb, plan.pair ? sm_count() / 2 : sm_count());
-  return static_cast<int>(ceil_div(kb, ceil_div(kb, split)));  // as make_geom: no empty split
+  return pick_slabs(o).slabs;
 }
 
 int gemm_bf16_slabs(const pom_gemm_args* a, int slabs, int* status, cudaStream_t st) {

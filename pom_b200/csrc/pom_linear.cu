@@ -188,21 +188,32 @@ __global__ void __launch_bounds__(32 * kFewWarps) linear_few_f32_kernel(const Fe
   }
 }
 
-// y = act(z + bias) + residual, elementwise over (M, N); y may be z itself.  VEC adjacent columns per thread.
+// y = act(z + bias) + residual over (M, N), z the sum of `slabs` fp32 matrices in their order; y may be the one slab.
+// VEC adjacent columns per thread.
 template <class T, int VEC>
-__global__ void __launch_bounds__(256) linear_epilogue_kernel(const FewDev a, const T* z, long long ldz, long long M) {
+__global__ void __launch_bounds__(256) linear_epilogue_kernel(const FewDev a, const float* z, long long ldz, int slabs,
+                                                              long long M) {
   griddep_wait();
   griddep_launch();
   const int per_row = a.N / VEC;
-  const long long total = M * per_row;
+  const long long total = M * per_row, each = M * ldz;
   for (long long i = blockIdx.x * 256ll + threadIdx.x; i < total; i += gridDim.x * 256ll) {
-    const long long r = i / per_row;
+    const long long r = total <= 0x7fffffff ? static_cast<unsigned>(i) / static_cast<unsigned>(per_row) : i / per_row;
     const int c = static_cast<int>(i - r * per_row) * VEC;
-    Piece<T, VEC> p, q;
-    p.raw = *reinterpret_cast<const typename Piece<T, VEC>::R*>(z + r * ldz + c);  // may alias y: no read-only path
+    Piece<float, VEC> in;
+    Piece<T, VEC> q;
+    // may be y: no read-only path
+    in.raw = *reinterpret_cast<const typename Piece<float, VEC>::R*>(z + r * ldz + c);
     float v[VEC], s[VEC];
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) v[e] = linear_act<true, Piece<T, 1>::kBf16>(a.act, p.get(e) + few_bias(a, c + e), s[e]);
+    for (int e = 0; e < VEC; ++e) v[e] = in.get(e);
+    for (int k = 1; k < slabs; ++k) {
+      in.ld(z + k * each + r * ldz + c);
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) v[e] += in.get(e);
+    }
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) v[e] = linear_act<true, Piece<T, 1>::kBf16>(a.act, v[e] + few_bias(a, c + e), s[e]);
     if (a.slope) {
       q.set(s);
       q.st(static_cast<T*>(a.slope) + r * a.ld_slope + c);
@@ -212,8 +223,8 @@ __global__ void __launch_bounds__(256) linear_epilogue_kernel(const FewDev a, co
 #pragma unroll
       for (int e = 0; e < VEC; ++e) v[e] += q.get(e);
     }
-    p.set(v);
-    p.st(static_cast<T*>(a.y) + r * a.ldy + c);
+    q.set(v);
+    q.st(static_cast<T*>(a.y) + r * a.ldy + c);
   }
 }
 
@@ -273,25 +284,6 @@ __global__ void __launch_bounds__(256) linear_dz_kernel(const T* __restrict__ dy
   }
 }
 
-// out = sum of the slabs, in their order, in the type T.
-template <class T>
-__global__ void __launch_bounds__(256) linear_slabs_kernel(const float* __restrict__ slabs, int count, long long each,
-                                                           T* __restrict__ out) {
-  griddep_wait();
-  griddep_launch();
-  for (long long i = (blockIdx.x * 256ll + threadIdx.x) * 4; i < each; i += gridDim.x * 1024ll) {
-    float4 s = __ldg(reinterpret_cast<const float4*>(slabs + i));
-    for (int k = 1; k < count; ++k) {
-      const float4 v = __ldg(reinterpret_cast<const float4*>(slabs + k * each + i));
-      s.x += v.x, s.y += v.y, s.z += v.z, s.w += v.w;
-    }
-    Piece<T, 4> p;
-    const float v[4] = {s.x, s.y, s.z, s.w};
-    p.set(v);
-    p.st(out + i);
-  }
-}
-
 int launched(cudaError_t e) {
   if (e != cudaSuccess) {
     (void)cudaGetLastError();
@@ -321,7 +313,8 @@ int check_linear(const pom_linear_args* a) {
   return POM_OK;
 }
 
-constexpr int kFewRowsBf16 = 64, kFewRowsF32 = 16;
+// bf16 1152 -> 4608: 8.1 us at 32 rows, 13.5 at 64, where the tensor cores take 11.5; 4608 -> 1152 at 64 rows: 19.7 and 12.3
+constexpr int kFewRowsBf16 = 32, kFewRowsF32 = 16;
 
 template <int MT>
 int launch_few_bf16(const FewDev& d, cudaStream_t st) {
@@ -347,9 +340,16 @@ int dz_chunk(int64_t M, int64_t N, int vec, bool sums_only) {
   return static_cast<int>(rows);
 }
 
+uint64_t up256(uint64_t v) { return (v + 255) / 256 * 256; }
+
+// Bytes of the slabs of a bf16 product with (M, N) outputs; 0: it is not cut.
+uint64_t slab_bytes(int slabs, int64_t M, int64_t N) {
+  return slabs > 1 ? up256(static_cast<uint64_t>(slabs) * M * N * 4) : 0;
+}
+
 struct BwdPlan {
-  int vec, chunk, chunks, slabs;
-  uint64_t dz, partial, slab, total;  // byte offsets into the workspace
+  int vec, chunk, chunks, dw_slabs, dx_slabs;
+  uint64_t dz, partial, slab, total;  // byte offsets into the workspace; the slabs of dw, then those of dx, lie at `slab`
 };
 
 BwdPlan bwd_plan(const pom_linear_args* a) {
@@ -358,17 +358,39 @@ BwdPlan bwd_plan(const pom_linear_args* a) {
   p.vec = a->N % per || a->ld_dy % per || !aligned16(a->dy) ? 1 : per;
   p.chunk = dz_chunk(a->M, a->N, p.vec, !a->slope);
   p.chunks = static_cast<int>(ceil_div(a->M, p.chunk));
-  p.slabs = a->dtype == POM_BF16 && a->dw ? gemm_bf16_slabs(a->N, a->K, a->M, true, true) : 1;
-  auto up = [](uint64_t v) { return (v + 255) / 256 * 256; };
+  const bool bf16 = a->dtype == POM_BF16;
+  p.dw_slabs = bf16 && a->dw ? gemm_bf16_slabs(a->N, a->K, a->M, true, true) : 1;
+  p.dx_slabs = bf16 && a->dx ? gemm_bf16_slabs(a->M, a->K, a->N, false, true) : 1;
   uint64_t at = 0;
   p.dz = at;
-  if (a->slope && !a->dz) at = up(at + static_cast<uint64_t>(a->M) * a->N * (a->dtype == POM_BF16 ? 2 : 4));
+  if (a->slope && !a->dz) at = up256(at + static_cast<uint64_t>(a->M) * a->N * (bf16 ? 2 : 4));
   p.partial = at;
-  if (a->dbias) at = up(at + static_cast<uint64_t>(p.chunks) * a->N * 4);
+  if (a->dbias) at = up256(at + static_cast<uint64_t>(p.chunks) * a->N * 4);
   p.slab = at;
-  if (p.slabs > 1) at = up(at + static_cast<uint64_t>(p.slabs) * a->N * a->K * 4);
-  p.total = at;
+  const uint64_t w = slab_bytes(p.dw_slabs, a->N, a->K), x = slab_bytes(p.dx_slabs, a->M, a->K);
+  p.total = at + (w > x ? w : x);
   return p;
+}
+
+// d.y = act(sum of slabs + bias) + residual in bf16 (T) or fp32.
+template <class T>
+int launch_epilogue(const FewDev& d, const float* z, int64_t ldz, int slabs, int64_t M, bool wide, cudaStream_t st) {
+  const int64_t want = ceil_div(M * (d.N / (wide ? 4 : 1)), 256), cap = 16ll * sm_count();
+  const dim3 grid(static_cast<unsigned>(want < cap ? want : cap));
+  const long long ld = ldz, rows = M;
+  return wide ? launched(launch_pdl(linear_epilogue_kernel<T, 4>, grid, dim3(256), 0, st, d, z, ld, slabs, rows))
+              : launched(launch_pdl(linear_epilogue_kernel<T, 1>, grid, dim3(256), 0, st, d, z, ld, slabs, rows));
+}
+
+// g, whose output is bf16 and contiguous, whole or as slabs and their sum.
+int product(pom_gemm_args g, int slabs, float* slab, int* status, cudaStream_t st) {
+  void* out = g.C;
+  if (slabs > 1) g.C = slab, g.out_mode = POM_OUT_F32;
+  const int rc = gemm_bf16_slabs(&g, slabs, status, st);
+  if (rc || slabs <= 1) return rc;
+  FewDev d{};
+  d.y = out, d.ldy = g.N, d.N = static_cast<int>(g.N);
+  return launch_epilogue<__nv_bfloat16>(d, slab, g.N, slabs, g.M, true, st);
 }
 
 // dz (where there is a slope) and dbias.
@@ -418,6 +440,19 @@ int pom_linear_fwd(const pom_linear_args* a, int* status, void* stream) {
   if (a->dtype != POM_BF16) return POM_ERR_UNSUPPORTED;  // pom_gemm_f32* and pom_linear_epilogue
   Operands o{a->x, a->w, a->M, a->N, a->K, a->ldx, a->ldw, 1, false, false};
   if ((rc = check_operands(o))) return rc;
+  const int slabs = gemm_bf16_slabs(a->M, a->N, a->K, false, false);
+  if (slabs > 1) {
+    if (!a->workspace) return POM_ERR_NULL;
+    if (a->N % 8 || a->ldy % 8 || (a->residual && a->ldr % 8)) return POM_ERR_BAD_STRIDE;
+    if (!aligned16(a->workspace) || !aligned16(a->y) || !aligned16(a->slope) || !aligned16(a->residual)) return POM_ERR_BAD_ALIGN;
+    pom_gemm_args g{};
+    g.A = a->x, g.Bm = a->w, g.C = a->workspace;
+    g.M = a->M, g.N = a->N, g.K = a->K;
+    g.lda = a->ldx, g.ldb = a->ldw, g.ldc = a->N;
+    g.batches = 1, g.split_k = 1, g.alpha = 1.f, g.out_mode = POM_OUT_F32;
+    if ((rc = gemm_bf16_slabs(&g, slabs, status, st))) return rc;
+    return launch_epilogue<__nv_bfloat16>(few_dev(a), static_cast<const float*>(a->workspace), a->N, slabs, a->M, true, st);
+  }
   EpiMaps maps{};
   if (a->slope && (rc = make_io_map(&maps.out0, a->slope, a->N, a->M, 1, a->N))) return rc;
   if ((rc = make_io_map(&maps.out1, a->y, a->N, a->M, 1, a->ldy))) return rc;
@@ -439,12 +474,12 @@ int pom_linear_epilogue(const pom_linear_args* a, const float* z, int64_t ldz, v
   const FewDev d = few_dev(a);
   const bool wide = a->N % 4 == 0 && ldz % 4 == 0 && a->ldy % 4 == 0 && aligned16(z) && aligned16(a->y) &&
                     aligned16(a->slope) && (!a->residual || (a->ldr % 4 == 0 && aligned16(a->residual)));
-  const int64_t want = ceil_div(a->M * (a->N / (wide ? 4 : 1)), 256), cap = 16ll * sm_count();
-  const dim3 grid(static_cast<unsigned>(want < cap ? want : cap));
-  cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const long long ld = ldz, M = a->M;
-  return wide ? launched(launch_pdl(linear_epilogue_kernel<float, 4>, grid, dim3(256), 0, st, d, z, ld, M))
-              : launched(launch_pdl(linear_epilogue_kernel<float, 1>, grid, dim3(256), 0, st, d, z, ld, M));
+  return launch_epilogue<float>(d, z, ldz, 1, a->M, wide, static_cast<cudaStream_t>(stream));
+}
+
+uint64_t pom_linear_fwd_workspace(const pom_linear_args* a) {
+  if (check_linear(a) || a->dtype != POM_BF16 || pom_linear_few_rows(a)) return 0;
+  return slab_bytes(gemm_bf16_slabs(a->M, a->N, a->K, false, false), a->M, a->N);
 }
 
 uint64_t pom_linear_bwd_workspace(const pom_linear_args* a) { return check_linear(a) ? 0 : bwd_plan(a).total; }
@@ -466,21 +501,14 @@ int pom_linear_bwd(const pom_linear_args* a, int* status, void* stream) {
   const int64_t ld_dz = a->slope ? a->N : a->ld_dy;
   pom_gemm_args g{};
   g.batches = 1, g.split_k = 1, g.alpha = 1.f;
+  float* slab = reinterpret_cast<float*>(ws + p.slab);
   if (a->dw) {
-    float* slabs = reinterpret_cast<float*>(ws + p.slab);
-    g.A = dz, g.Bm = a->x, g.C = p.slabs > 1 ? static_cast<void*>(slabs) : a->dw;
+    g.A = dz, g.Bm = a->x, g.C = a->dw;
     g.M = a->N, g.N = a->K, g.K = a->M;
     g.lda = ld_dz, g.ldb = a->ldx, g.ldc = a->K;
     g.a_mn_major = g.b_mn_major = 1;
-    g.out_mode = p.slabs > 1 ? POM_OUT_F32 : POM_OUT_BF16;
-    if ((rc = gemm_bf16_slabs(&g, p.slabs, status, st))) return rc;
-    if (p.slabs > 1) {
-      const int64_t each = a->N * a->K, want = ceil_div(each, 1024), cap = 8ll * sm_count();
-      if ((rc = launched(launch_pdl(linear_slabs_kernel<__nv_bfloat16>, dim3(static_cast<unsigned>(want < cap ? want : cap)), dim3(256), 0,
-                                    st, static_cast<const float*>(slabs), p.slabs, static_cast<long long>(each),
-                                    static_cast<__nv_bfloat16*>(a->dw)))))
-        return rc;
-    }
+    g.out_mode = POM_OUT_BF16;
+    if ((rc = product(g, p.dw_slabs, slab, status, st))) return rc;
   }
   if (a->dx) {
     g.A = dz, g.Bm = a->w, g.C = a->dx;
@@ -488,7 +516,7 @@ int pom_linear_bwd(const pom_linear_args* a, int* status, void* stream) {
     g.lda = ld_dz, g.ldb = a->ldw, g.ldc = a->K;
     g.a_mn_major = 0, g.b_mn_major = 1;
     g.out_mode = POM_OUT_BF16;
-    if ((rc = pom_gemm_bf16(&g, status, st))) return rc;
+    if ((rc = product(g, p.dx_slabs, slab, status, st))) return rc;
   }
   return check_launch();
 }
