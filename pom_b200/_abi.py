@@ -303,7 +303,6 @@ _SIGNATURES = {
     "pom_layer_norm_bwd_workspace": (C.c_uint64, [C.POINTER(LayerNormArgs)]),
     "pom_layer_norm_bwd": (C.c_int, [C.POINTER(LayerNormArgs), C.c_void_p]),
     "pom_linear_few_rows": (C.c_int, [C.POINTER(LinearArgs)]),
-    "pom_linear_fwd_workspace": (C.c_uint64, [C.POINTER(LinearArgs)]),
     "pom_linear_fwd": (C.c_int, [C.POINTER(LinearArgs), C.c_void_p, C.c_void_p]),
     "pom_linear_epilogue": (C.c_int, [C.POINTER(LinearArgs), C.c_void_p, C.c_int64, C.c_void_p]),
     "pom_linear_bwd_workspace": (C.c_uint64, [C.POINTER(LinearArgs)]),

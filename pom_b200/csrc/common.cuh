@@ -74,8 +74,8 @@ inline cudaError_t launch_pdl(Kern kern, dim3 grid, dim3 block, size_t smem, cud
 // `tile_weight` gives 0 (one batch, no K split): those k-blocks are left out (pom_gemm.cu).
 int gemm_bf16_dead_k(const pom_gemm_args* a, const float* tile_weight, int dead_k, int* status, cudaStream_t st);
 
-// A bf16 product with a long K and few output tiles (a weight gradient, or few rows), cut along K without atomics: the
-// first form says into how many slabs a product of these sizes is cut, the second writes every slab's fp32 sums at
+// A bf16 product with a long K and few output tiles (a weight gradient), cut along K without atomics: the first form says
+// into how many slabs a product of these sizes is cut, the second writes every slab's fp32 sums at
 // C + slab * M * ldc (one slab: any output mode, as pom_gemm_bf16).
 int gemm_bf16_slabs(int64_t M, int64_t N, int64_t K, bool a_mn, bool b_mn);
 int gemm_bf16_slabs(const pom_gemm_args* a, int slabs, int* status, cudaStream_t st);

@@ -23,12 +23,11 @@ struct SlabPlan {
   int slabs;
 };
 
-// Whether a product is worth cutting along K into slabs that a second kernel adds, and how.  Estimated time in
-// microseconds: 4 for the launch and the filling of the pipeline, per wave 1 for its epilogue and, per 64 of K, what one
-// tile takes to arrive in shared memory (about 64 bytes a cycle and SM, which bounds a tile before its MMAs do; measured
-// 0.285 / 0.37 / 0.335 for 128 and 256 columns of one CTA and 256 of a pair), and for slabs 3 for the second launch and
-// their traffic at 6 TB/s.  Measured against one slab: 512 x 1152 x 4608 24.6 -> 13.7 us before the second kernel (4
-// slabs), 256 x 1024 x 4096 21.9 -> 9.2 (8); 2048 x 1024 x 4096 24.3 -> 20.8 (2), which the second kernel undoes: stays whole.
+// Into how many slabs along K a weight gradient is cut, and by which tiles.  Estimated time in microseconds: per wave 1 for its
+// epilogue and, per 64 of K, what one tile takes to arrive in shared memory (about 64 bytes a cycle and SM, which bounds a
+// tile before its MMAs do; measured 0.285 / 0.37 / 0.335 for 128 and 256 columns of one CTA and 256 of a pair), and for
+// slabs 3 for the second launch and their traffic at 6 TB/s.  4608 x 1152 over 32768 rows: three slabs, 264 us and 17 for
+// their sum; 512 x 1152 over 4608: 24.6 us whole, 13.7 in four slabs and 3 for the sum.
 SlabPlan pick_slabs(const Operands& o) {
   struct Cand {
     bool pair;

@@ -3,10 +3,11 @@
 //   forward   z = x W^T + bias, y = act(z) + residual, slope = act'(z) (kept for a backward pass)
 //   backward  dz = dy * slope;  dx = dz W;  dW = dz^T x;  dbias = sum of dz over the rows;  dresidual = dy
 //
-// bf16, many rows: the tcgen05 GEMM engine with EpiLinear.  Few rows: linear_few_*_kernel, which reads the weight once
-// and spreads it over all SMs.  float32 with many rows: the caller runs pom_gemm_f32 / pom_gemm_f32_planes and
+// bf16, many rows: the tcgen05 GEMM engine with EpiLinear, or, where that leaves SMs idle, clusters that share a tile
+// (gemm_cluster.cuh).  Few rows: linear_few_*_kernel, which reads the weight once and spreads it over all SMs.  float32 with many rows: the caller runs pom_gemm_f32 / pom_gemm_f32_planes and
 // pom_linear_epilogue.  Sums are fp32; nothing here is summed by atomics, so a call gives the same bits every time.
 #include "epilogues_linear.cuh"
+#include "gemm_cluster.cuh"
 #include "gemm_launch.cuh"
 #include "rows.cuh"
 
@@ -348,8 +349,8 @@ uint64_t slab_bytes(int slabs, int64_t M, int64_t N) {
 }
 
 struct BwdPlan {
-  int vec, chunk, chunks, dw_slabs, dx_slabs;
-  uint64_t dz, partial, slab, total;  // byte offsets into the workspace; the slabs of dw, then those of dx, lie at `slab`
+  int vec, chunk, chunks, dw_slabs;
+  uint64_t dz, partial, slab, total;  // byte offsets into the workspace
 };
 
 BwdPlan bwd_plan(const pom_linear_args* a) {
@@ -360,15 +361,13 @@ BwdPlan bwd_plan(const pom_linear_args* a) {
   p.chunks = static_cast<int>(ceil_div(a->M, p.chunk));
   const bool bf16 = a->dtype == POM_BF16;
   p.dw_slabs = bf16 && a->dw ? gemm_bf16_slabs(a->N, a->K, a->M, true, true) : 1;
-  p.dx_slabs = bf16 && a->dx ? gemm_bf16_slabs(a->M, a->K, a->N, false, true) : 1;
   uint64_t at = 0;
   p.dz = at;
   if (a->slope && !a->dz) at = up256(at + static_cast<uint64_t>(a->M) * a->N * (bf16 ? 2 : 4));
   p.partial = at;
   if (a->dbias) at = up256(at + static_cast<uint64_t>(p.chunks) * a->N * 4);
   p.slab = at;
-  const uint64_t w = slab_bytes(p.dw_slabs, a->N, a->K), x = slab_bytes(p.dx_slabs, a->M, a->K);
-  p.total = at + (w > x ? w : x);
+  p.total = at + slab_bytes(p.dw_slabs, a->N, a->K);
   return p;
 }
 
@@ -440,18 +439,16 @@ int pom_linear_fwd(const pom_linear_args* a, int* status, void* stream) {
   if (a->dtype != POM_BF16) return POM_ERR_UNSUPPORTED;  // pom_gemm_f32* and pom_linear_epilogue
   Operands o{a->x, a->w, a->M, a->N, a->K, a->ldx, a->ldw, 1, false, false};
   if ((rc = check_operands(o))) return rc;
-  const int slabs = gemm_bf16_slabs(a->M, a->N, a->K, false, false);
-  if (slabs > 1) {
-    if (!a->workspace) return POM_ERR_NULL;
+  const ClusterPlan cp = pick_cluster(a->M, a->N, a->K);
+  if (cp.size > 1) {
     if (a->N % 8 || a->ldy % 8 || (a->residual && a->ldr % 8)) return POM_ERR_BAD_STRIDE;
-    if (!aligned16(a->workspace) || !aligned16(a->y) || !aligned16(a->slope) || !aligned16(a->residual)) return POM_ERR_BAD_ALIGN;
-    pom_gemm_args g{};
-    g.A = a->x, g.Bm = a->w, g.C = a->workspace;
-    g.M = a->M, g.N = a->N, g.K = a->K;
-    g.lda = a->ldx, g.ldb = a->ldw, g.ldc = a->N;
-    g.batches = 1, g.split_k = 1, g.alpha = 1.f, g.out_mode = POM_OUT_F32;
-    if ((rc = gemm_bf16_slabs(&g, slabs, status, st))) return rc;
-    return launch_epilogue<__nv_bfloat16>(few_dev(a), static_cast<const float*>(a->workspace), a->N, slabs, a->M, true, st);
+    if (!aligned16(a->y) || !aligned16(a->slope) || !aligned16(a->residual)) return POM_ERR_BAD_ALIGN;
+    ClusterDev d{};
+    d.bias = a->bias, d.bias_f32 = a->bias_dtype == POM_F32, d.act = a->act;
+    d.residual = static_cast<const __nv_bfloat16*>(a->residual), d.ldr = a->ldr;
+    d.y = static_cast<__nv_bfloat16*>(a->y), d.ldy = a->ldy;
+    d.slope = static_cast<__nv_bfloat16*>(a->slope);
+    return cluster_product(o, cp, d, status, st);
   }
   EpiMaps maps{};
   if (a->slope && (rc = make_io_map(&maps.out0, a->slope, a->N, a->M, 1, a->N))) return rc;
@@ -475,11 +472,6 @@ int pom_linear_epilogue(const pom_linear_args* a, const float* z, int64_t ldz, v
   const bool wide = a->N % 4 == 0 && ldz % 4 == 0 && a->ldy % 4 == 0 && aligned16(z) && aligned16(a->y) &&
                     aligned16(a->slope) && (!a->residual || (a->ldr % 4 == 0 && aligned16(a->residual)));
   return launch_epilogue<float>(d, z, ldz, 1, a->M, wide, static_cast<cudaStream_t>(stream));
-}
-
-uint64_t pom_linear_fwd_workspace(const pom_linear_args* a) {
-  if (check_linear(a) || a->dtype != POM_BF16 || pom_linear_few_rows(a)) return 0;
-  return slab_bytes(gemm_bf16_slabs(a->M, a->N, a->K, false, false), a->M, a->N);
 }
 
 uint64_t pom_linear_bwd_workspace(const pom_linear_args* a) { return check_linear(a) ? 0 : bwd_plan(a).total; }
@@ -516,7 +508,16 @@ int pom_linear_bwd(const pom_linear_args* a, int* status, void* stream) {
     g.lda = ld_dz, g.ldb = a->ldw, g.ldc = a->K;
     g.a_mn_major = 0, g.b_mn_major = 1;
     g.out_mode = POM_OUT_BF16;
-    if ((rc = product(g, p.dx_slabs, slab, status, st))) return rc;
+    const ClusterPlan cp = pick_cluster(a->M, a->K, a->N);
+    if (cp.size > 1) {
+      Operands o{dz, a->w, a->M, a->K, a->N, ld_dz, a->ldw, 1, false, true};
+      ClusterDev d{};
+      d.y = static_cast<__nv_bfloat16*>(a->dx), d.ldy = a->K;
+      rc = cluster_product(o, cp, d, status, st);
+    } else {
+      rc = pom_gemm_bf16(&g, status, st);
+    }
+    if (rc) return rc;
   }
   return check_launch();
 }

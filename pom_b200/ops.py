@@ -1063,10 +1063,6 @@ def linear_fwd(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor], a
         a.residual = residual.data_ptr()
     L = _abi.lib()
     if bf16 or L.pom_linear_few_rows(C.byref(a)):
-        nbytes = L.pom_linear_fwd_workspace(C.byref(a))
-        if nbytes:
-            ws = x.new_empty(nbytes, dtype=torch.uint8)
-            a.workspace = ws.data_ptr()
         _abi.check(L.pom_linear_fwd(C.byref(a), _abi.status_word(x.device).data_ptr(), _abi.stream_ptr()), "pom_linear_fwd")
         return y, slope
     gemm(x.as_strided((M, K), (ldx, 1)), w.as_strided((N, K), (ldw, 1)), out=y.view(M, N))
