@@ -666,20 +666,19 @@ enum { POM_ACT_NONE = 0, POM_ACT_GELU = 1, POM_ACT_GELU_TANH = 2, POM_ACT_SILU =
 
 /* y = act(x w^T + bias) + residual with x (M, K), w (N, K), bias (N), residual and y (M, N).
  *
- * Forward (pom_linear_fwd): slope, where given, receives act'(x w^T + bias) as contiguous (M, N) values of dtype: what
- * the backward call needs of the forward pass.  bf16: K, N and every row stride multiples of 8, 16-byte aligned addresses.  float32: only calls for which pom_linear_few_rows is nonzero; for the others z = x w^T comes from
- * pom_gemm_f32 or pom_gemm_f32_planes, and pom_linear_epilogue does the rest (y may be z).
- *
- * Backward (pom_linear_bwd): dz = dy * slope (slope NULL: dz = dy), dbias = column sums of dz, dw = dz^T x (N, K) and
- * dx = dz w (M, K), both contiguous; any of the three may be NULL.  dz: NULL, or where to put it (contiguous).  float32:
- * dz and dbias only (dx and dw NULL).  workspace: pom_linear_bwd_workspace bytes, 16-byte aligned. */
+ * Forward: z, where given, receives x w^T + bias as contiguous (M, N) values of dtype: what the backward call of a product
+ * with an activation needs.  Backward: dz = dy act'(z) (no activation: dz = dy, z unused), dbias = column sums of dz,
+ * dw = dz^T x (N, K) and dx = dz w (M, K), both contiguous; any of the three may be NULL.  dz: NULL, or where to put it
+ * (contiguous).  workspace: as many bytes as the _workspace calls say (often 0 forward), 16-byte aligned.
+ * bf16: K, N and every row stride multiples of 8, 16-byte aligned addresses.  float32: any; fma nonzero keeps the products
+ * on the FMA kernel, which needs no workspace for planes of the operands. */
 typedef struct pom_linear_args {
   const void* x;
   const void* w;
   const void* bias;
   const void* residual;
   void* y;
-  void* slope;
+  void* z;
   const void* dy;
   void* dz;
   void* dx;
@@ -688,11 +687,10 @@ typedef struct pom_linear_args {
   void* workspace;
   int64_t M, N, K;
   int64_t ldx, ldw, ldr, ldy, ld_dy;
-  int32_t act, dtype, bias_dtype, reserved0;
+  int32_t act, dtype, bias_dtype, fma;
 } pom_linear_args;
-int pom_linear_few_rows(const pom_linear_args* a);
+uint64_t pom_linear_fwd_workspace(const pom_linear_args* a);
 int pom_linear_fwd(const pom_linear_args* a, int* status, void* stream);
-int pom_linear_epilogue(const pom_linear_args* a, const float* z, int64_t ldz, void* stream);
 uint64_t pom_linear_bwd_workspace(const pom_linear_args* a);
 int pom_linear_bwd(const pom_linear_args* a, int* status, void* stream);
 

@@ -197,12 +197,12 @@ ACTIVATIONS = {None: 0, "gelu": 1, "gelu_tanh": 2, "silu": 3, "relu": 4}
 class LinearArgs(C.Structure):
     _fields_ = [
         ("x", C.c_void_p), ("w", C.c_void_p), ("bias", C.c_void_p), ("residual", C.c_void_p), ("y", C.c_void_p),
-        ("slope", C.c_void_p),
+        ("z", C.c_void_p),
         ("dy", C.c_void_p), ("dz", C.c_void_p), ("dx", C.c_void_p), ("dw", C.c_void_p), ("dbias", C.c_void_p),
         ("workspace", C.c_void_p),
         ("M", C.c_int64), ("N", C.c_int64), ("K", C.c_int64),
         ("ldx", C.c_int64), ("ldw", C.c_int64), ("ldr", C.c_int64), ("ldy", C.c_int64), ("ld_dy", C.c_int64),
-        ("act", C.c_int32), ("dtype", C.c_int32), ("bias_dtype", C.c_int32), ("reserved0", C.c_int32),
+        ("act", C.c_int32), ("dtype", C.c_int32), ("bias_dtype", C.c_int32), ("fma", C.c_int32),
     ]
 
 
@@ -302,9 +302,8 @@ _SIGNATURES = {
     "pom_layer_norm_fwd": (C.c_int, [C.POINTER(LayerNormArgs), C.c_void_p]),
     "pom_layer_norm_bwd_workspace": (C.c_uint64, [C.POINTER(LayerNormArgs)]),
     "pom_layer_norm_bwd": (C.c_int, [C.POINTER(LayerNormArgs), C.c_void_p]),
-    "pom_linear_few_rows": (C.c_int, [C.POINTER(LinearArgs)]),
+    "pom_linear_fwd_workspace": (C.c_uint64, [C.POINTER(LinearArgs)]),
     "pom_linear_fwd": (C.c_int, [C.POINTER(LinearArgs), C.c_void_p, C.c_void_p]),
-    "pom_linear_epilogue": (C.c_int, [C.POINTER(LinearArgs), C.c_void_p, C.c_int64, C.c_void_p]),
     "pom_linear_bwd_workspace": (C.c_uint64, [C.POINTER(LinearArgs)]),
     "pom_linear_bwd": (C.c_int, [C.POINTER(LinearArgs), C.c_void_p, C.c_void_p]),
     "pom_rope_axes": (C.c_int, [C.POINTER(RopeAxesArgs), C.c_void_p]),
@@ -376,6 +375,12 @@ def status_word(device) -> torch.Tensor:
     if key not in _status:
         _status[key] = torch.zeros(1, dtype=torch.int32, device=device)
     return _status[key]
+
+
+def status_ptr(index: int) -> int:
+    """Address of the status word of CUDA device ``index``."""
+    word = _status.get(index)
+    return (status_word(torch.device("cuda", index)) if word is None else word).data_ptr()
 
 
 def read_status(device) -> int:

@@ -123,18 +123,19 @@ class _Linear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, residual, act):
         nx, nw, nb, _, _ = ctx.needs_input_grad
-        y, slope = ops.linear_fwd(x, weight, bias, act, residual, act is not None and (nx or nw or nb))
-        ctx.save_for_backward(x, weight, slope)
+        y, z = ops.linear_fwd(x, weight, bias, act, residual, act is not None and (nx or nw or nb))
+        ctx.save_for_backward(x, weight, z)
+        ctx.act = act
         ctx.bias_dtype = bias.dtype if nb else None
         return y
 
     @_backward
     def backward(ctx, g):
-        x, weight, slope = ctx.saved_tensors
+        x, weight, z = ctx.saved_tensors
         nx, nw, nb, nr, _ = ctx.needs_input_grad
         dx = dw = db = None
         if nx or nw or nb:
-            dx, dw, db = ops.linear_bwd(g, x, weight, slope, want_dx=nx, want_dw=nw, bias_dtype=ctx.bias_dtype)
+            dx, dw, db = ops.linear_bwd(g, x, weight, ctx.act, z, want_dx=nx, want_dw=nw, bias_dtype=ctx.bias_dtype)
         return dx, dw, db, (g if nr else None), None
 
 
@@ -149,8 +150,8 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] =
 
     x (..., K) and ``weight`` (N, K) of one dtype, bfloat16 or float32; ``bias`` (N,) in that dtype or float32;
     ``residual`` of the output's shape and dtype; ``activation`` None, "gelu" (exact), "gelu_tanh", "silu" or "relu".
-    Sums, bias, activation and residual are float32, rounded once.  With an activation and a gradient to come, its slope
-    is kept in x's dtype and the backward pass multiplies by it.  bfloat16 widths that are not multiples of 8 are padded
+    Sums, bias, activation and residual are float32, rounded once.  With an activation and a gradient to come, its argument
+    is kept in x's dtype.  bfloat16 widths that are not multiples of 8 are padded
     with zeros (a copy of the operands).  Under ``torch.autocast("cuda", torch.bfloat16)`` x, ``weight`` and ``residual``
     are cast to bfloat16 on the way in."""
     _check_tokens(x)

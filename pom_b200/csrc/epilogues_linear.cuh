@@ -1,63 +1,32 @@
-// Epilogue of the linear operator on the tcgen05 GEMM engine: y = act(acc + bias) + residual, and, for a backward pass,
-// the slope act'(acc + bias) beside it.
+// Epilogue of the linear operator on the tcgen05 GEMM engine: y = act(z) + residual with z = acc + bias, and, for a backward
+// pass, z beside it.
 //
-// The slope is kept instead of the pre-activation: both cost one bf16 per element, but with the slope the backward pass
-// is a product (dz = dy * slope) where the pre-activation would need the derivative again from its rounded value.
-// Rounding the slope to bf16 (half a step, 2^-9 of its value) puts the same relative error into dz as rounding dz itself,
-// which the tensor cores need anyway.
+// z is kept rounded to bf16 and its slope formed again in the backward pass: an error of 2^-9 in z moves the slope by that
+// times |z| act''(z), a quarter of what rounding the slope itself would do.  What remains is the rounding of dz, which the
+// tensor cores need.
 #pragma once
 #include "epilogues.cuh"
-#include "f32x2.cuh"
 #include "linear_math.cuh"
 
 namespace pomk {
 
-// 32 values of a row: v becomes act(v), and with SLOPE ps the packed act'(v).
-template <int ACT, bool SLOPE>
-__device__ __forceinline__ void linear_act32(float (&v)[32], uint32_t (&ps)[16]) {
+template <int ACT>
+__device__ __forceinline__ void linear_act32(float (&v)[32]) {
 #pragma unroll
   for (int i = 0; i < 32; i += 2) {
-    float s0, s1;
-    v[i] = linear_act<SLOPE, true>(ACT, v[i], s0);
-    v[i + 1] = linear_act<SLOPE, true>(ACT, v[i + 1], s1);
-    if (SLOPE) ps[i / 2] = pack_bf16x2(s0, s1);
-  }
-}
-
-// gelu of 32 values in packed pairs: the arithmetic of linear_act<SLOPE, true>.
-template <bool SLOPE>
-__device__ __forceinline__ void gelu32(float (&v)[32], uint32_t (&ps)[16]) {
-#pragma unroll
-  for (int i = 0; i < 32; i += 2) {
-    const F2 z(v[i], v[i + 1]);
-    const F2 d = fma2(F2(fabsf(z.v.x), fabsf(z.v.y)), F2(0.2316418882f), F2(1.f));
-    const F2 t(fast_rcp(d.v.x), fast_rcp(d.v.y));
-    const F2 w = mul2(mul2(z, F2(-0.72134752044f)), z);
-    const F2 e(fast_exp2(w.v.x), fast_exp2(w.v.y));
-    F2 q = fma2(F2(0.5307027145f), t, F2(-0.7265760135f));
-    q = fma2(q, t, F2(0.7107068705f));
-    q = fma2(q, t, F2(-0.142248368f));
-    q = fma2(q, t, F2(0.127414796f));
-    q = mul2(q, mul2(t, e));
-    const F2 up = fma2(q, F2(-1.f), F2(1.f));
-    const F2 phi(z.v.x < 0.f ? q.v.x : up.v.x, z.v.y < 0.f ? q.v.y : up.v.y);
-    if (SLOPE) {
-      const F2 s = fma2(mul2(z, F2(0.3989422804014327f)), e, phi);
-      ps[i / 2] = pack_bf16x2(s.v.x, s.v.y);
-    }
-    const F2 y = mul2(z, phi);
+    const F2 y = linear_act2<true>(ACT, F2(v[i], v[i + 1]));
     v[i] = y.v.x, v[i + 1] = y.v.y;
   }
 }
 
-template <bool SLOPE>
-__device__ __forceinline__ void linear_act32(int act, float (&v)[32], uint32_t (&ps)[16]) {
+// 32 values of a row; the choice of the activation stands outside their loop.
+__device__ __forceinline__ void linear_act32(int act, float (&v)[32]) {
   switch (act) {
-    case POM_ACT_GELU: gelu32<SLOPE>(v, ps); break;
-    case POM_ACT_GELU_TANH: linear_act32<POM_ACT_GELU_TANH, SLOPE>(v, ps); break;
-    case POM_ACT_SILU: linear_act32<POM_ACT_SILU, SLOPE>(v, ps); break;
-    case POM_ACT_RELU: linear_act32<POM_ACT_RELU, SLOPE>(v, ps); break;
-    default: linear_act32<POM_ACT_NONE, SLOPE>(v, ps); break;
+    case POM_ACT_GELU: linear_act32<POM_ACT_GELU>(v); break;
+    case POM_ACT_GELU_TANH: linear_act32<POM_ACT_GELU_TANH>(v); break;
+    case POM_ACT_SILU: linear_act32<POM_ACT_SILU>(v); break;
+    case POM_ACT_RELU: linear_act32<POM_ACT_RELU>(v); break;
+    default: break;
   }
 }
 
@@ -67,10 +36,10 @@ struct EpiLinear {
     const void* bias;  // (N) bf16 or fp32, or null
     int bias_f32;
     int act;
-    int save_slope;  // maps.out0 = slope; maps.out1 = y; maps.in0 = residual
+    int save_z;  // maps.out0 = z; maps.out1 = y; maps.in0 = residual
   };
   static constexpr int kSmemBytes = 2 * 256 * 4;  // double-buffered bias
-  // per warp: [slope or y][y], with a residual [residual in][y][slope]
+  // per warp: [z or y][y], with a residual [residual in][y][z or y]
   static constexpr int kStageBytes = RES ? 6144 : 4096;
   static constexpr bool kStager = false;
   template <int BN>
@@ -129,12 +98,11 @@ struct EpiLinear {
         const float4 b = *reinterpret_cast<const float4*>(cst + c * 32 + i);
         v[i] += b.x, v[i + 1] += b.y, v[i + 2] += b.z, v[i + 3] += b.w;
       }
-      if (p.save_slope) {
-        linear_act32<true>(p.act, v, pk);
+      if (p.save_z) {
+        pack32(v, pk);
         if (t.rows_valid > 0) store_block<1>(RES ? base + 4096 : base, &maps.out0, pk, lane, col, y, t.b);
-      } else {
-        linear_act32<false>(p.act, v, pk);
       }
+      linear_act32(p.act, v);
       if constexpr (RES) {
         float r[32];
         if (alive) alive = mbar_wait(io.bar, io.load_phase, io.abort_flag, io.status, kStatusEpilogueTimeout);
@@ -149,8 +117,8 @@ struct EpiLinear {
       }
       pack32(v, pk);
       if (t.rows_valid > 0) {
-        // with a slope the two stores use one block each; without one, y alternates between two blocks
-        uint8_t* out = RES ? base + (p.save_slope || !flip ? 2048 : 4096) : (p.save_slope || flip ? base + 2048 : base);
+        // with z the two stores use one block each; without it, y alternates between two blocks
+        uint8_t* out = RES ? base + (p.save_z || !flip ? 2048 : 4096) : (p.save_z || flip ? base + 2048 : base);
         store_block<1>(out, &maps.out1, pk, lane, col, y, t.b);
       }
       flip ^= 1;

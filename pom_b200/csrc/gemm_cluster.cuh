@@ -6,7 +6,7 @@
 // while a few of them read.  A cluster of `size` CTAs divides that time by `size`.  Every CTA owns BN / size columns of the
 // result: it sends the other columns of its partial tile to their owners (st.shared::cluster, 512 adjacent bytes a warp: with
 // the rows apart, the same stores took 4 us instead of 1), and after one cluster barrier adds what it has received to its own
-// accumulator, in the order of the ranks: the same bits on every run.  Then bias, activation, slope and residual, from
+// accumulator, in the order of the ranks: the same bits on every run.  Then bias, activation and residual, from
 // registers to global memory; bias and residual are fetched while the main loop runs.
 //
 // Roles and waits as in gemm_sm100.cuh: warp 0 loads, warp 1 issues the MMAs, warps 2 to 9 are the epilogue; every wait on
@@ -21,7 +21,7 @@ struct ClusterDev {
   const void* bias;  // (N) bf16 or fp32, or null
   const __nv_bfloat16* residual;
   __nv_bfloat16* y;
-  __nv_bfloat16* slope;  // contiguous, or null
+  __nv_bfloat16* z;  // contiguous, or null
   long long ldr, ldy;
   int bias_f32, act;
   int M, N, m_tiles, k_blocks;
@@ -237,18 +237,25 @@ gemm_cluster_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
         const float4 b = *reinterpret_cast<const float4*>(bias_sm + p * 16 + k);
         v[k] += b.x, v[k + 1] += b.y, v[k + 2] += b.z, v[k + 3] += b.w;
       }
-      float sl[16];
+      if (a.z && r < a.M) {
 #pragma unroll
-      for (int k = 0; k < 16; ++k) v[k] = linear_act<true, true>(a.act, v[k], sl[k]);
+        for (int h = 0; h < 2; ++h)
+          if (col + 8 * h < a.N) {
+            const float* t = v + 8 * h;
+            *reinterpret_cast<uint4*>(a.z + r * a.N + col + 8 * h) =
+                make_uint4(pack_bf16x2(t[0], t[1]), pack_bf16x2(t[2], t[3]), pack_bf16x2(t[4], t[5]), pack_bf16x2(t[6], t[7]));
+          }
+      }
+#pragma unroll
+      for (int k = 0; k < 16; k += 2) {
+        const F2 y = linear_act2<true>(a.act, F2(v[k], v[k + 1]));
+        v[k] = y.v.x, v[k + 1] = y.v.y;
+      }
       if (r < a.M) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           const int c = col + 8 * h;
           if (c < a.N) {
-            const float* t = sl + 8 * h;
-            if (a.slope)
-              *reinterpret_cast<uint4*>(a.slope + r * a.N + c) =
-                  make_uint4(pack_bf16x2(t[0], t[1]), pack_bf16x2(t[2], t[3]), pack_bf16x2(t[4], t[5]), pack_bf16x2(t[6], t[7]));
             float* u = v + 8 * h;
             const uint32_t w[4] = {res[i][h].x, res[i][h].y, res[i][h].z, res[i][h].w};
 #pragma unroll

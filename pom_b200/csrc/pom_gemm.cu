@@ -26,8 +26,8 @@ struct SlabPlan {
 // Into how many slabs along K a weight gradient is cut, and by which tiles.  Estimated time in microseconds: per wave 1 for its
 // epilogue and, per 64 of K, what one tile takes to arrive in shared memory (about 64 bytes a cycle and SM, which bounds a
 // tile before its MMAs do; measured 0.285 / 0.37 / 0.335 for 128 and 256 columns of one CTA and 256 of a pair), and for
-// slabs 3 for the second launch and their traffic at 6 TB/s.  4608 x 1152 over 32768 rows: three slabs, 264 us and 17 for
-// their sum; 512 x 1152 over 4608: 24.6 us whole, 13.7 in four slabs and 3 for the sum.
+// slabs 3 for the second launch and their reading at 6 TB/s.  4608 x 1152 over 32768 rows: four slabs, 264 us and 16 for
+// their sum (three: 283 and 15); 512 x 1152 over 4608: 24.6 us whole, 13.7 in four slabs and 3 for the sum.
 SlabPlan pick_slabs(const Operands& o) {
   struct Cand {
     bool pair;
@@ -36,7 +36,7 @@ SlabPlan pick_slabs(const Operands& o) {
   };
   const Cand cands[3] = {{true, 256, 0.335}, {false, 256, 0.37}, {false, 128, 0.285}};
   const long long kb = ceil_div(o.K, kBK);
-  const double slab_us = static_cast<double>(o.M) * static_cast<double>(o.N) * 8.0 / 6e6;
+  const double slab_us = static_cast<double>(o.M) * static_cast<double>(o.N) * 4.0 / 6e6;  // read again; written beside the MMAs
   SlabPlan best{TilePlan{true, 256}, 1};
   double best_cost = -1.0;
   for (const Cand& c : cands) {

@@ -1,11 +1,13 @@
 // The linear operator: y = act(x W^T + bias) + residual, and its backward pass.
 //
-//   forward   z = x W^T + bias, y = act(z) + residual, slope = act'(z) (kept for a backward pass)
-//   backward  dz = dy * slope;  dx = dz W;  dW = dz^T x;  dbias = sum of dz over the rows;  dresidual = dy
+//   forward   z = x W^T + bias (kept for a backward pass), y = act(z) + residual
+//   backward  dz = dy act'(z);  dx = dz W;  dW = dz^T x;  dbias = sum of dz over the rows;  dresidual = dy
 //
 // bf16, many rows: the tcgen05 GEMM engine with EpiLinear, or, where that leaves SMs idle, clusters that share a tile
-// (gemm_cluster.cuh).  Few rows: linear_few_*_kernel, which reads the weight once and spreads it over all SMs.  float32 with many rows: the caller runs pom_gemm_f32 / pom_gemm_f32_planes and
-// pom_linear_epilogue.  Sums are fp32; nothing here is summed by atomics, so a call gives the same bits every time.
+// (gemm_cluster.cuh).  Few rows: linear_few_*_kernel, which reads the weight once and spreads it over all SMs.
+// float32 with more rows: the products of pom_gemm_f32_planes or pom_gemm_f32, and linear_epilogue_kernel.
+//
+// Sums are fp32; nothing here is summed by atomics, so a call gives the same bits every time.
 #include "epilogues_linear.cuh"
 #include "gemm_cluster.cuh"
 #include "gemm_launch.cuh"
@@ -18,8 +20,8 @@ namespace {
 
 struct FewDev {
   const void *x, *w, *bias, *residual;
-  void *y, *slope;
-  long long ldx, ldw, ldr, ldy, ld_slope;
+  void *y, *z;  // z (contiguous) or null
+  long long ldx, ldw, ldr, ldy;
   int M, N, K, act, bias_f32;
 };
 
@@ -41,16 +43,12 @@ template <class T>
 __device__ __forceinline__ void few_finish(const FewDev& a, int row, int n, float z) {
   Piece<T, 1> p;
   z += few_bias(a, n);
-  float v[1];
-  if (a.slope) {
-    float s[1];
-    v[0] = linear_act<true, Piece<T, 1>::kBf16>(a.act, z, s[0]);
-    p.set(s);
-    p.st(static_cast<T*>(a.slope) + row * a.ld_slope + n);
-  } else {
-    float none;
-    v[0] = linear_act<false, Piece<T, 1>::kBf16>(a.act, z, none);
+  if (a.z) {
+    const float k[1] = {z};
+    p.set(k);
+    p.st(static_cast<T*>(a.z) + static_cast<long long>(row) * a.N + n);
   }
+  float v[1] = {linear_act<Piece<T, 1>::kBf16>(a.act, z)};
   if (a.residual) {
     p.ld(static_cast<const T*>(a.residual) + row * a.ldr + n);
     v[0] += p.get(0);
@@ -198,6 +196,7 @@ __global__ void __launch_bounds__(256) linear_epilogue_kernel(const FewDev a, co
   griddep_launch();
   const int per_row = a.N / VEC;
   const long long total = M * per_row, each = M * ldz;
+  const bool wide_bias = a.bias && !(reinterpret_cast<uintptr_t>(a.bias) & 15);
   for (long long i = blockIdx.x * 256ll + threadIdx.x; i < total; i += gridDim.x * 256ll) {
     const long long r = total <= 0x7fffffff ? static_cast<unsigned>(i) / static_cast<unsigned>(per_row) : i / per_row;
     const int c = static_cast<int>(i - r * per_row) * VEC;
@@ -205,7 +204,7 @@ __global__ void __launch_bounds__(256) linear_epilogue_kernel(const FewDev a, co
     Piece<T, VEC> q;
     // may be y: no read-only path
     in.raw = *reinterpret_cast<const typename Piece<float, VEC>::R*>(z + r * ldz + c);
-    float v[VEC], s[VEC];
+    float v[VEC];
 #pragma unroll
     for (int e = 0; e < VEC; ++e) v[e] = in.get(e);
     for (int k = 1; k < slabs; ++k) {
@@ -213,12 +212,27 @@ __global__ void __launch_bounds__(256) linear_epilogue_kernel(const FewDev a, co
 #pragma unroll
       for (int e = 0; e < VEC; ++e) v[e] += in.get(e);
     }
+    if (wide_bias) {
+      if (a.bias_f32) {
+        in.ld(static_cast<const float*>(a.bias) + c);
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) v[e] = linear_act<true, Piece<T, 1>::kBf16>(a.act, v[e] + few_bias(a, c + e), s[e]);
-    if (a.slope) {
-      q.set(s);
-      q.st(static_cast<T*>(a.slope) + r * a.ld_slope + c);
+        for (int e = 0; e < VEC; ++e) v[e] += in.get(e);
+      } else {
+        Piece<__nv_bfloat16, VEC> b;
+        b.ld(static_cast<const __nv_bfloat16*>(a.bias) + c);
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) v[e] += b.get(e);
+      }
+    } else if (a.bias) {
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) v[e] += few_bias(a, c + e);
     }
+    if (a.z) {
+      q.set(v);
+      q.st(static_cast<T*>(a.z) + r * a.N + c);
+    }
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) v[e] = linear_act<Piece<T, 1>::kBf16>(a.act, v[e]);
     if (a.residual) {
       q.ld(static_cast<const T*>(a.residual) + r * a.ldr + c);
 #pragma unroll
@@ -229,12 +243,13 @@ __global__ void __launch_bounds__(256) linear_epilogue_kernel(const FewDev a, co
   }
 }
 
-// dz = dy * slope (no slope: dz = dy, which is not written) and the column sums of dz over the block's rows.
+// dz = dy act'(z) (ACT none: dz = dy, which is not written) and the column sums of dz over the block's rows.
 // Block = 32 column lanes of VEC columns x 8 row lanes; grid = (column blocks, row chunks).
-template <class T, int VEC>
-__global__ void __launch_bounds__(256) linear_dz_kernel(const T* __restrict__ dy, long long ld_dy, const T* __restrict__ slope,
+template <class T, int VEC, int ACT>
+__global__ void __launch_bounds__(256) linear_dz_kernel(const T* __restrict__ dy, long long ld_dy, const T* __restrict__ z,
                                                         T* __restrict__ dz, float* __restrict__ partial, long long M, int N,
                                                         int chunk) {
+  constexpr bool kFast = Piece<T, 1>::kBf16;
   __shared__ float sm[8][32 * VEC + 1];
   griddep_wait();
   griddep_launch();
@@ -246,25 +261,36 @@ __global__ void __launch_bounds__(256) linear_dz_kernel(const T* __restrict__ dy
 #pragma unroll
   for (int e = 0; e < VEC; ++e) acc[e] = 0.f;
   if (c < N) {
-    constexpr int U = 4;
+    // rows in flight: with gelu in bf16 147 us at two (32768 x 4608) and 151 at four, in float32 18.1 and 16.7 (4079 x 1536)
+    constexpr int U = kFast ? 2 : 4;
     for (long long r = r0 + ty; r < r1; r += 8 * U) {
-      Piece<T, VEC> g[U], s[U];
+      Piece<T, VEC> g[U], p[U];
 #pragma unroll
       for (int u = 0; u < U; ++u)
         if (r + 8 * u < r1) {
           g[u].ld(dy + (r + 8 * u) * ld_dy + c);
-          if (slope) s[u].ld(slope + (r + 8 * u) * N + c);
+          if (ACT != POM_ACT_NONE) p[u].ld(z + (r + 8 * u) * N + c);
         }
 #pragma unroll
       for (int u = 0; u < U; ++u)
         if (r + 8 * u < r1) {
           float v[VEC];
+          if constexpr (ACT == POM_ACT_NONE) {
 #pragma unroll
-          for (int e = 0; e < VEC; ++e) {
-            v[e] = slope ? g[u].get(e) * s[u].get(e) : g[u].get(e);
-            acc[e] += v[e];
+            for (int e = 0; e < VEC; ++e) v[e] = g[u].get(e);
+          } else if constexpr (VEC == 1) {
+            v[0] = g[u].get(0) * linear_slope2<kFast>(ACT, F2(p[u].get(0), 0.f)).v.x;
+          } else {
+#pragma unroll
+            for (int e = 0; e < VEC; e += 2) {
+              const F2 s = linear_slope2<kFast>(ACT, F2(p[u].get(e), p[u].get(e + 1)));
+              const F2 d = mul2(s, F2(g[u].get(e), g[u].get(e + 1)));
+              v[e] = d.v.x, v[e + 1] = d.v.y;
+            }
           }
-          if (slope) {
+#pragma unroll
+          for (int e = 0; e < VEC; ++e) acc[e] += v[e];
+          if (ACT != POM_ACT_NONE) {
             g[u].set(v);
             g[u].st(dz + (r + 8 * u) * N + c);
           }
@@ -297,8 +323,8 @@ int launched(cudaError_t e) {
 FewDev few_dev(const pom_linear_args* a) {
   FewDev d;
   d.x = a->x, d.w = a->w, d.bias = a->bias, d.residual = a->residual;
-  d.y = a->y, d.slope = a->slope;
-  d.ldx = a->ldx, d.ldw = a->ldw, d.ldr = a->ldr, d.ldy = a->ldy, d.ld_slope = a->N;
+  d.y = a->y, d.z = a->z;
+  d.ldx = a->ldx, d.ldw = a->ldw, d.ldr = a->ldr, d.ldy = a->ldy;
   d.M = static_cast<int>(a->M < INT32_MAX ? a->M : INT32_MAX), d.N = static_cast<int>(a->N), d.K = static_cast<int>(a->K);
   d.act = a->act, d.bias_f32 = a->bias_dtype == POM_F32;
   return d;
@@ -348,26 +374,64 @@ uint64_t slab_bytes(int slabs, int64_t M, int64_t N) {
   return slabs > 1 ? up256(static_cast<uint64_t>(slabs) * M * N * 4) : 0;
 }
 
+bool few_rows(const pom_linear_args* a) {
+  const int per = a->dtype == POM_BF16 ? 8 : 4;
+  return a->M <= (a->dtype == POM_BF16 ? kFewRowsBf16 : kFewRowsF32) && a->K % per == 0 && a->ldx % per == 0 &&
+         a->ldw % per == 0 && aligned16(a->x) && aligned16(a->w);
+}
+
+// A float32 product on the tensor cores: three bf16 planes of each operand and the partial sums of a cut product, one after
+// the other in a workspace.  total 0: on the FMA kernel.
+struct F32Plan {
+  uint64_t b, scratch, total;
+};
+
+// A holds a_rows x a_cols values as it is stored, B b_rows x b_cols.
+F32Plan f32_plan(const pom_linear_args* a, int64_t M, int64_t N, int64_t K, int out_mode, int64_t a_rows, int64_t a_cols,
+                 int64_t b_rows, int64_t b_cols) {
+  F32Plan p{};
+  // Short sums run on the FMA kernel (see f32_planes_pay of the Python layer), and so do small products with sums of up to
+  // 512 terms: one launch instead of three, which is what such a call waits for (500 x 300 -> 700 in training 139 us
+  // against 174), while a longer chain would lose digits that a blocked sum keeps.
+  if (a->fma || K < 128 || (K <= 512 && static_cast<double>(M) * static_cast<double>(N) * static_cast<double>(K) < 0x1p27)) return p;
+  p.b = up256(pom_f32_planes_bytes(a_rows, a_cols));
+  p.scratch = p.b + up256(pom_f32_planes_bytes(b_rows, b_cols));
+  p.total = p.scratch + up256(pom_gemm_f32_planes_scratch(M, N, K, out_mode));
+  return p;
+}
+
+int f32_product(const pom_gemm_args& g, const F32Plan& p, char* ws, int a_ready, int* status, cudaStream_t st) {
+  if (!p.total) return pom_gemm_f32(&g, st);
+  return pom_gemm_f32_planes(&g, ws, a_ready, ws + p.b, 0, ws + p.scratch, status, st);
+}
+
 struct BwdPlan {
   int vec, chunk, chunks, dw_slabs;
-  uint64_t dz, partial, slab, total;  // byte offsets into the workspace
+  uint64_t dz, partial, slab, total;  // byte offsets into the workspace; float32: the planes at `slab`
+  F32Plan dw32, dx32;                 // A = dz in both: its planes are made once
 };
 
 BwdPlan bwd_plan(const pom_linear_args* a) {
   BwdPlan p{};
   const int per = a->dtype == POM_BF16 ? 8 : 4;
   p.vec = a->N % per || a->ld_dy % per || !aligned16(a->dy) ? 1 : per;
-  p.chunk = dz_chunk(a->M, a->N, p.vec, !a->slope);
+  p.chunk = dz_chunk(a->M, a->N, p.vec, a->act == POM_ACT_NONE);
   p.chunks = static_cast<int>(ceil_div(a->M, p.chunk));
   const bool bf16 = a->dtype == POM_BF16;
   p.dw_slabs = bf16 && a->dw ? gemm_bf16_slabs(a->N, a->K, a->M, true, true) : 1;
   uint64_t at = 0;
   p.dz = at;
-  if (a->slope && !a->dz) at = up256(at + static_cast<uint64_t>(a->M) * a->N * (bf16 ? 2 : 4));
+  if (a->act != POM_ACT_NONE && !a->dz) at = up256(at + static_cast<uint64_t>(a->M) * a->N * (bf16 ? 2 : 4));
   p.partial = at;
   if (a->dbias) at = up256(at + static_cast<uint64_t>(p.chunks) * a->N * 4);
   p.slab = at;
   p.total = at + slab_bytes(p.dw_slabs, a->N, a->K);
+  if (!bf16) {
+    // dw sums over the rows and has few output tiles: it is accumulated, since only that may be cut along its sum
+    if (a->dw) p.dw32 = f32_plan(a, a->N, a->K, a->M, POM_OUT_F32_ACCUM, a->M, a->N, a->M, a->K);
+    if (a->dx) p.dx32 = f32_plan(a, a->M, a->K, a->N, POM_OUT_F32, a->M, a->N, a->N, a->K);
+    p.total = at + (p.dw32.total > p.dx32.total ? p.dw32.total : p.dx32.total);
+  }
   return p;
 }
 
@@ -392,19 +456,34 @@ int product(pom_gemm_args g, int slabs, float* slab, int* status, cudaStream_t s
   return launch_epilogue<__nv_bfloat16>(d, slab, g.N, slabs, g.M, true, st);
 }
 
-// dz (where there is a slope) and dbias.
-int dz_and_bias(const pom_linear_args* a, const BwdPlan& p, void* dz, cudaStream_t st) {
-  if (!a->slope && !a->dbias) return POM_OK;
-  float* partial = a->dbias ? reinterpret_cast<float*>(static_cast<char*>(a->workspace) + p.partial) : nullptr;
-  const dim3 grid(static_cast<unsigned>(ceil_div(a->N, 32 * p.vec)), static_cast<unsigned>(p.chunks));
+template <class T, int VEC>
+int launch_dz(const pom_linear_args* a, const BwdPlan& p, void* dz, float* partial, cudaStream_t st) {
+  const dim3 grid(static_cast<unsigned>(ceil_div(a->N, 32 * VEC)), static_cast<unsigned>(p.chunks));
   const long long M = a->M, ld = a->ld_dy;
   const int N = static_cast<int>(a->N);
-#define POM_DZ(T, V)                                                                                                    \
-  launched(launch_pdl(linear_dz_kernel<T, V>, grid, dim3(256), 0, st, static_cast<const T*>(a->dy), ld,                 \
-                      static_cast<const T*>(a->slope), static_cast<T*>(dz), partial, M, N, p.chunk))
-  int rc = a->dtype == POM_BF16 ? (p.vec == 8 ? POM_DZ(__nv_bfloat16, 8) : POM_DZ(__nv_bfloat16, 1))
-                                : (p.vec == 4 ? POM_DZ(float, 4) : POM_DZ(float, 1));
+#define POM_DZ(ACT)                                                                                                     \
+  case ACT:                                                                                                             \
+    return launched(launch_pdl(linear_dz_kernel<T, VEC, ACT>, grid, dim3(256), 0, st, static_cast<const T*>(a->dy), ld, \
+                               static_cast<const T*>(a->z), static_cast<T*>(dz), partial, M, N, p.chunk));
+  switch (a->act) {
+    POM_DZ(POM_ACT_NONE)
+    POM_DZ(POM_ACT_GELU)
+    POM_DZ(POM_ACT_GELU_TANH)
+    POM_DZ(POM_ACT_SILU)
+    POM_DZ(POM_ACT_RELU)
+  }
 #undef POM_DZ
+  return POM_ERR_UNSUPPORTED;
+}
+
+// dz (with an activation) and dbias.
+int dz_and_bias(const pom_linear_args* a, const BwdPlan& p, void* dz, cudaStream_t st) {
+  if (a->act == POM_ACT_NONE && !a->dbias) return POM_OK;
+  float* partial = a->dbias ? reinterpret_cast<float*>(static_cast<char*>(a->workspace) + p.partial) : nullptr;
+  const int N = static_cast<int>(a->N);
+  const int rc = a->dtype == POM_BF16
+                     ? (p.vec == 8 ? launch_dz<__nv_bfloat16, 8>(a, p, dz, partial, st) : launch_dz<__nv_bfloat16, 1>(a, p, dz, partial, st))
+                     : (p.vec == 4 ? launch_dz<float, 4>(a, p, dz, partial, st) : launch_dz<float, 1>(a, p, dz, partial, st));
   if (rc || !partial) return rc;
   return sum_rows(partial, p.chunks, N, N, a->bias_dtype, a->dbias, nullptr, st);
 }
@@ -413,20 +492,13 @@ int dz_and_bias(const pom_linear_args* a, const BwdPlan& p, void* dz, cudaStream
 
 extern "C" {
 
-int pom_linear_few_rows(const pom_linear_args* a) {
-  if (check_linear(a)) return 0;
-  const int per = a->dtype == POM_BF16 ? 8 : 4;
-  return a->M <= (a->dtype == POM_BF16 ? kFewRowsBf16 : kFewRowsF32) && a->K % per == 0 && a->ldx % per == 0 &&
-         a->ldw % per == 0 && aligned16(a->x) && aligned16(a->w);
-}
-
 int pom_linear_fwd(const pom_linear_args* a, int* status, void* stream) {
   int rc = check_linear(a);
   if (rc) return rc;
   if (!a->x || !a->w || !a->y) return POM_ERR_NULL;
   if (a->ldx < a->K || a->ldw < a->K || a->ldy < a->N || (a->residual && a->ldr < a->N)) return POM_ERR_BAD_STRIDE;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (pom_linear_few_rows(a)) {
+  if (few_rows(a)) {
     const FewDev d = few_dev(a);
     if (a->dtype == POM_BF16) {
       return a->M <= 16 ? launch_few_bf16<1>(d, st) : launch_few_bf16<2>(d, st);
@@ -436,42 +508,49 @@ int pom_linear_fwd(const pom_linear_args* a, int* status, void* stream) {
     if (a->M <= 8) return launch_few_f32<8>(d, st);
     return launch_few_f32<16>(d, st);
   }
-  if (a->dtype != POM_BF16) return POM_ERR_UNSUPPORTED;  // pom_gemm_f32* and pom_linear_epilogue
+  if (a->dtype == POM_F32) {
+    const F32Plan p = f32_plan(a, a->M, a->N, a->K, POM_OUT_F32, a->M, a->K, a->N, a->K);
+    if (p.total && !a->workspace) return POM_ERR_NULL;
+    if (!aligned16(a->workspace)) return POM_ERR_BAD_ALIGN;
+    pom_gemm_args g{};
+    g.A = a->x, g.Bm = a->w, g.C = a->y;
+    g.M = a->M, g.N = a->N, g.K = a->K;
+    g.lda = a->ldx, g.ldb = a->ldw, g.ldc = a->ldy;
+    g.batches = 1, g.split_k = 1, g.alpha = 1.f, g.out_mode = POM_OUT_F32;
+    if ((rc = f32_product(g, p, static_cast<char*>(a->workspace), 0, status, st))) return rc;
+    if (!a->bias && !a->residual && !a->z && a->act == POM_ACT_NONE) return POM_OK;
+    const bool wide = a->N % 4 == 0 && a->ldy % 4 == 0 && aligned16(a->y) && aligned16(a->z) &&
+                      (!a->residual || (a->ldr % 4 == 0 && aligned16(a->residual)));
+    return launch_epilogue<float>(few_dev(a), static_cast<const float*>(a->y), a->ldy, 1, a->M, wide, st);
+  }
   Operands o{a->x, a->w, a->M, a->N, a->K, a->ldx, a->ldw, 1, false, false};
   if ((rc = check_operands(o))) return rc;
   const ClusterPlan cp = pick_cluster(a->M, a->N, a->K);
   if (cp.size > 1) {
     if (a->N % 8 || a->ldy % 8 || (a->residual && a->ldr % 8)) return POM_ERR_BAD_STRIDE;
-    if (!aligned16(a->y) || !aligned16(a->slope) || !aligned16(a->residual)) return POM_ERR_BAD_ALIGN;
+    if (!aligned16(a->y) || !aligned16(a->z) || !aligned16(a->residual)) return POM_ERR_BAD_ALIGN;
     ClusterDev d{};
     d.bias = a->bias, d.bias_f32 = a->bias_dtype == POM_F32, d.act = a->act;
     d.residual = static_cast<const __nv_bfloat16*>(a->residual), d.ldr = a->ldr;
     d.y = static_cast<__nv_bfloat16*>(a->y), d.ldy = a->ldy;
-    d.slope = static_cast<__nv_bfloat16*>(a->slope);
+    d.z = static_cast<__nv_bfloat16*>(a->z);
     return cluster_product(o, cp, d, status, st);
   }
   EpiMaps maps{};
-  if (a->slope && (rc = make_io_map(&maps.out0, a->slope, a->N, a->M, 1, a->N))) return rc;
+  if (a->z && (rc = make_io_map(&maps.out0, a->z, a->N, a->M, 1, a->N))) return rc;
   if ((rc = make_io_map(&maps.out1, a->y, a->N, a->M, 1, a->ldy))) return rc;
   if (a->residual) {
     if ((rc = make_io_map(&maps.in0, a->residual, a->N, a->M, 1, a->ldr))) return rc;
-    const EpiLinear<true>::Params ep{a->bias, a->bias_dtype == POM_F32, a->act, a->slope != nullptr};
+    const EpiLinear<true>::Params ep{a->bias, a->bias_dtype == POM_F32, a->act, a->z != nullptr};
     return run_plan<false, false, EpiLinear<true>>(pick_plan(o, true), o, 1, maps, ep, status, st);
   }
-  const EpiLinear<false>::Params ep{a->bias, a->bias_dtype == POM_F32, a->act, a->slope != nullptr};
+  const EpiLinear<false>::Params ep{a->bias, a->bias_dtype == POM_F32, a->act, a->z != nullptr};
   return run_plan<false, false, EpiLinear<false>>(pick_plan(o, true), o, 1, maps, ep, status, st);
 }
 
-int pom_linear_epilogue(const pom_linear_args* a, const float* z, int64_t ldz, void* stream) {
-  int rc = check_linear(a);
-  if (rc) return rc;
-  if (!z || !a->y) return POM_ERR_NULL;
-  if (a->dtype != POM_F32) return POM_ERR_UNSUPPORTED;
-  if (ldz < a->N || a->ldy < a->N || (a->residual && a->ldr < a->N)) return POM_ERR_BAD_STRIDE;
-  const FewDev d = few_dev(a);
-  const bool wide = a->N % 4 == 0 && ldz % 4 == 0 && a->ldy % 4 == 0 && aligned16(z) && aligned16(a->y) &&
-                    aligned16(a->slope) && (!a->residual || (a->ldr % 4 == 0 && aligned16(a->residual)));
-  return launch_epilogue<float>(d, z, ldz, 1, a->M, wide, static_cast<cudaStream_t>(stream));
+uint64_t pom_linear_fwd_workspace(const pom_linear_args* a) {
+  if (check_linear(a) || a->dtype != POM_F32 || few_rows(a)) return 0;
+  return f32_plan(a, a->M, a->N, a->K, POM_OUT_F32, a->M, a->K, a->N, a->K).total;
 }
 
 uint64_t pom_linear_bwd_workspace(const pom_linear_args* a) { return check_linear(a) ? 0 : bwd_plan(a).total; }
@@ -479,7 +558,7 @@ uint64_t pom_linear_bwd_workspace(const pom_linear_args* a) { return check_linea
 int pom_linear_bwd(const pom_linear_args* a, int* status, void* stream) {
   int rc = check_linear(a);
   if (rc) return rc;
-  if (!a->dy || (a->dw && !a->x) || (a->dx && !a->w)) return POM_ERR_NULL;
+  if (!a->dy || (a->act != POM_ACT_NONE && !a->z) || (a->dw && !a->x) || (a->dx && !a->w)) return POM_ERR_NULL;
   if (a->ld_dy < a->N || (a->dx && a->ldw < a->K) || (a->dw && a->ldx < a->K)) return POM_ERR_BAD_STRIDE;
   const BwdPlan p = bwd_plan(a);
   if (p.total && !a->workspace) return POM_ERR_NULL;
@@ -488,28 +567,37 @@ int pom_linear_bwd(const pom_linear_args* a, int* status, void* stream) {
   char* ws = static_cast<char*>(a->workspace);
   void* own_dz = a->dz ? a->dz : ws + p.dz;
   if ((rc = dz_and_bias(a, p, own_dz, st))) return rc;
-  if (a->dtype != POM_BF16) return a->dx || a->dw ? POM_ERR_UNSUPPORTED : POM_OK;
-  const void* dz = a->slope ? own_dz : a->dy;
-  const int64_t ld_dz = a->slope ? a->N : a->ld_dy;
+  const bool own = a->act != POM_ACT_NONE;
+  const void* dz = own ? own_dz : a->dy;
+  const int64_t ld_dz = own ? a->N : a->ld_dy;
   pom_gemm_args g{};
   g.batches = 1, g.split_k = 1, g.alpha = 1.f;
-  float* slab = reinterpret_cast<float*>(ws + p.slab);
+  const bool f32 = a->dtype == POM_F32;
   if (a->dw) {
     g.A = dz, g.Bm = a->x, g.C = a->dw;
     g.M = a->N, g.N = a->K, g.K = a->M;
     g.lda = ld_dz, g.ldb = a->ldx, g.ldc = a->K;
     g.a_mn_major = g.b_mn_major = 1;
-    g.out_mode = POM_OUT_BF16;
-    if ((rc = product(g, p.dw_slabs, slab, status, st))) return rc;
+    if (f32) {
+      g.out_mode = p.dw32.total ? POM_OUT_F32_ACCUM : POM_OUT_F32;
+      if (p.dw32.total && (rc = pom_fill_zero(a->dw, a->N * a->K * 4, st))) return rc;
+      rc = f32_product(g, p.dw32, ws + p.slab, 0, status, st);
+    } else {
+      g.out_mode = POM_OUT_BF16;
+      rc = product(g, p.dw_slabs, reinterpret_cast<float*>(ws + p.slab), status, st);
+    }
+    if (rc) return rc;
   }
   if (a->dx) {
     g.A = dz, g.Bm = a->w, g.C = a->dx;
     g.M = a->M, g.N = a->K, g.K = a->N;
     g.lda = ld_dz, g.ldb = a->ldw, g.ldc = a->K;
     g.a_mn_major = 0, g.b_mn_major = 1;
-    g.out_mode = POM_OUT_BF16;
-    const ClusterPlan cp = pick_cluster(a->M, a->K, a->N);
-    if (cp.size > 1) {
+    g.out_mode = f32 ? POM_OUT_F32 : POM_OUT_BF16;
+    const ClusterPlan cp = f32 ? ClusterPlan{128, 1} : pick_cluster(a->M, a->K, a->N);
+    if (f32) {
+      rc = f32_product(g, p.dx32, ws + p.slab, p.dw32.total != 0, status, st);
+    } else if (cp.size > 1) {
       Operands o{dz, a->w, a->M, a->K, a->N, ld_dz, a->ldw, 1, false, true};
       ClusterDev d{};
       d.y = static_cast<__nv_bfloat16*>(a->dx), d.ldy = a->K;

@@ -1038,9 +1038,29 @@ def _linear_args(x, w, act, M, N, K, ldx, ldw) -> LinearArgs:
     return a
 
 
+def _linear_workspace(size, a: LinearArgs, x: torch.Tensor) -> Optional[torch.Tensor]:
+    """Workspace of as many bytes as ``size`` asks for.  Where memory has no room for the planes of float32 operands, the
+    FMA kernel, which needs none."""
+    nbytes = size(C.byref(a))
+    if not nbytes:
+        return None
+    try:
+        ws = x.new_empty(nbytes, dtype=torch.uint8)
+    except torch.OutOfMemoryError:
+        if x.dtype != torch.float32:
+            raise
+        a.fma = 1
+        nbytes = size(C.byref(a))
+        if not nbytes:
+            return None
+        ws = x.new_empty(nbytes, dtype=torch.uint8)
+    a.workspace = ws.data_ptr()
+    return ws
+
+
 def linear_fwd(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor], act: Optional[str],
-               residual: Optional[torch.Tensor], want_slope: bool):
-    """act(x·wᵀ + bias) + residual: (y, slope), slope (M, N) = act'(x·wᵀ + bias) or None.  x (..., K), w (N, K), both bf16
+               residual: Optional[torch.Tensor], want_z: bool):
+    """act(z) + residual with z = x·wᵀ + bias: (y, z), z (M, N) in x's dtype or None.  x (..., K), w (N, K), both bf16
     (K and N multiples of 8) or both float32; ``bias`` contiguous, bf16 or float32."""
     _same_device(x, w, bias, residual)
     bf16 = x.dtype == torch.bfloat16
@@ -1049,32 +1069,29 @@ def linear_fwd(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor], a
     N, K = w.shape
     M = x.numel() // K
     y = x.new_empty((*x.shape[:-1], N))
-    slope = x.new_empty((M, N)) if want_slope else None
+    z = x.new_empty((M, N)) if want_z else None
     if M == 0:
-        return y, slope
+        return y, z
     a = _linear_args(x, w, act, M, N, K, ldx, ldw)
     a.y, a.ldy = y.data_ptr(), N
     if bias is not None:
         a.bias, a.bias_dtype = bias.data_ptr(), _DTYPE[bias.dtype]
-    if slope is not None:
-        a.slope = slope.data_ptr()
+    if z is not None:
+        a.z = z.data_ptr()
     if residual is not None:
         residual, a.ldr = rows_of(residual, bf16)
         a.residual = residual.data_ptr()
     L = _abi.lib()
-    if bf16 or L.pom_linear_few_rows(C.byref(a)):
-        _abi.check(L.pom_linear_fwd(C.byref(a), _abi.status_word(x.device).data_ptr(), _abi.stream_ptr()), "pom_linear_fwd")
-        return y, slope
-    gemm(x.as_strided((M, K), (ldx, 1)), w.as_strided((N, K), (ldw, 1)), out=y.view(M, N))
-    if bias is not None or residual is not None or act is not None:
-        _abi.check(L.pom_linear_epilogue(C.byref(a), a.y, N, _abi.stream_ptr()), "pom_linear_epilogue")
-    return y, slope
+    if not bf16:
+        ws = _linear_workspace(L.pom_linear_fwd_workspace, a, x)  # noqa: F841 (alive until the call below)
+    _abi.check(L.pom_linear_fwd(C.byref(a), _abi.status_ptr(x.get_device()), _abi.stream_ptr()), "pom_linear_fwd")
+    return y, z
 
 
-def linear_bwd(dy: torch.Tensor, x: torch.Tensor, w: torch.Tensor, slope: Optional[torch.Tensor], *, want_dx: bool,
-               want_dw: bool, bias_dtype: Optional[torch.dtype]):
+def linear_bwd(dy: torch.Tensor, x: torch.Tensor, w: torch.Tensor, act: Optional[str], z: Optional[torch.Tensor], *,
+               want_dx: bool, want_dw: bool, bias_dtype: Optional[torch.dtype]):
     """(dx, dw, dbias) of :func:`linear_fwd` (dbias where ``bias_dtype`` is given); what is not wanted is None."""
-    _same_device(dy, x, w, slope)
+    _same_device(dy, x, w, z)
     bf16 = x.dtype == torch.bfloat16
     x, ldx = rows_of(x, bf16)
     w, ldw = rows_of(w, bf16)
@@ -1086,35 +1103,19 @@ def linear_bwd(dy: torch.Tensor, x: torch.Tensor, w: torch.Tensor, slope: Option
     if M == 0:
         return dx, dw if dw is None else fill_zero(dw), db if db is None else fill_zero(db)
     dy, ldg = rows_of(dy, bf16)
-    a = _linear_args(x, w, None, M, N, K, ldx, ldw)
+    a = _linear_args(x, w, act, M, N, K, ldx, ldw)
     a.dy, a.ld_dy = dy.data_ptr(), ldg
-    if slope is not None:
-        a.slope = slope.data_ptr()
+    if z is not None:
+        a.z = z.data_ptr()
     if db is not None:
         a.dbias, a.bias_dtype = db.data_ptr(), _DTYPE[bias_dtype]
-    dz = None
-    if bf16:
-        a.dx, a.dw = ptr(dx), ptr(dw)
-    elif slope is not None:
-        dz = torch.empty_like(slope)
-        a.dz = dz.data_ptr()
+    if dx is not None:
+        a.dx = dx.data_ptr()
+    if dw is not None:
+        a.dw = dw.data_ptr()
     L = _abi.lib()
-    nbytes = L.pom_linear_bwd_workspace(C.byref(a))
-    if nbytes:
-        ws = x.new_empty(nbytes, dtype=torch.uint8)
-        a.workspace = ws.data_ptr()
-    _abi.check(L.pom_linear_bwd(C.byref(a), _abi.status_word(x.device).data_ptr(), _abi.stream_ptr()), "pom_linear_bwd")
-    if not bf16:
-        if dz is None:
-            dz = dy.as_strided((M, N), (ldg, 1))
-        planes = F32Planes()  # of dz, which enters both products
-        if want_dw:
-            # a sum over many rows with few output tiles: only an accumulated product is cut along its sum
-            cut = f32_planes_pay(M)
-            gemm(dz, x.as_strided((M, K), (ldx, 1)), a_mn=True, b_mn=True, out=fill_zero(dw) if cut else dw, accumulate=cut,
-                 a_planes=planes)
-        if want_dx:
-            gemm(dz, w.as_strided((N, K), (ldw, 1)), b_mn=True, out=dx.view(M, K), a_planes=planes)
+    ws = _linear_workspace(L.pom_linear_bwd_workspace, a, x)  # noqa: F841 (alive until the call below)
+    _abi.check(L.pom_linear_bwd(C.byref(a), _abi.status_ptr(x.get_device()), _abi.stream_ptr()), "pom_linear_bwd")
     return dx, dw, db
 
 

@@ -95,12 +95,21 @@ def test_the_library_refuses_bad_arguments_before_it_launches():
     assert L.pom_linear_fwd(ctypes.byref(m), None, None) == -2  # ldy
     m.ldy, m.act = 8, 9
     assert L.pom_linear_fwd(ctypes.byref(m), None, None) == -4
-    m.act, m.dtype, m.M = 0, 1, 1000
-    assert L.pom_linear_few_rows(ctypes.byref(m)) == 0
-    assert L.pom_linear_fwd(ctypes.byref(m), None, None) == -4  # float32 with many rows
-    m.M, m.dtype, m.K, m.ldx, m.ldw = 4, 0, 12, 12, 12
-    assert L.pom_linear_few_rows(ctypes.byref(m)) == 0
+    m.act, m.dtype, m.M, m.K, m.ldx, m.ldw = 0, 1, 1000, 256, 256, 256
+    assert L.pom_linear_fwd_workspace(ctypes.byref(m)) >= 6 * (1000 * 256 + 8 * 256)
+    assert L.pom_linear_fwd(ctypes.byref(m), None, None) == -8  # float32 operands without room for their planes
+    m.fma = 1
+    assert L.pom_linear_fwd_workspace(ctypes.byref(m)) == 0
+    m.fma = m.dtype = 0
+    m.M, m.K, m.ldx, m.ldw = 4, 12, 12, 12
     assert L.pom_linear_fwd(ctypes.byref(m), None, None) == -2  # rows that bulk copies cannot address
+    m.M, m.K, m.ldx, m.ldw, m.ld_dy, m.act = 64, 64, 64, 64, 8, 1
+    assert L.pom_linear_bwd(ctypes.byref(m), None, None) == -8  # no dy
+    m.dy = 16
+    assert L.pom_linear_bwd(ctypes.byref(m), None, None) == -8  # an activation without its argument
+    m.z = 16
+    assert L.pom_linear_bwd_workspace(ctypes.byref(m)) >= 64 * 8 * 2
+    assert L.pom_linear_bwd(ctypes.byref(m), None, None) == -8  # no workspace
     assert L.pom_rope_axes(ctypes.byref(r), None) == -8
     r.x = r.y = r.pos = 16
     assert L.pom_rope_axes(ctypes.byref(r), None) == -4

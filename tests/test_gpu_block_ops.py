@@ -176,8 +176,8 @@ def linear_check(x, w, b, r, act, dy, label=""):
     if r is not None:
         want = a + r.detach().double().reshape(M, N)
     within(y.detach().reshape(M, N), want, ye + E * want.abs(), label + "y")
-    # the slope changes by at most 1 per unit of z (relu: any amount within ze of 0), and is stored
-    se = 0 if act is None else ze + h * s.abs() + 16 * E * (z.abs() + 1)
+    # the slope, which changes by at most 0.8 per unit of z (relu: any amount within ze of 0), is taken at the stored z
+    se = 0 if act is None else 0.8 * (ze + h * z.abs()) + 16 * E * (z.abs() + 1)
     if act == "relu":
         se = se + (z.abs() <= ze).double()
     dz = g * s
