@@ -124,6 +124,9 @@ struct EpiStore {
     const bool row_ok = row < t.rows_valid;
     const long long off = static_cast<long long>(t.b) * p.batch_stride + static_cast<long long>(t.row0 + row) * p.ldc +
                           static_cast<long long>(t.split) * p.split_stride;
+    // the two store blocks alternate anew in every tile, and a 192-column tile ends on the block it began with: the store of
+    // the tile before must have left it
+    if (lane == 0) bulk_wait_read<0>();
     int flip = 0;
 #pragma unroll 1
     for (int c = half; c < BN / 32; c += kEpiColSplit) {
