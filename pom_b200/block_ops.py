@@ -6,6 +6,9 @@ The reference leaves these to ``torch.nn`` (its README builds the blocks around 
 float32 tensors, any strides (rows that do not follow one another in one step are copied), run on the tensors' device
 and current stream, are differentiable once, and may be captured into CUDA graphs.  They give the same bits on every
 run.  ``pom_b200.operators`` exports them.
+
+A backward pass is captured together with its forward pass, and, as with PyTorch's own operators, while no eager graph of
+the same leaves is alive (autograd would join the capture with the stream that such a graph was made on; it raises).
 """
 from __future__ import annotations
 
@@ -197,12 +200,13 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] =
 class _RotateAxes(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, pos, tables):
-        ctx.pos, ctx.tables = pos, tables
+        ctx.save_for_backward(pos, *(t for pair in tables for t in pair))  # an update in place before backward is noticed
         return ops.rope_axes(x, pos, tables)
 
     @_backward
     def backward(ctx, g):
-        return ops.rope_axes(g, ctx.pos, ctx.tables, transpose=True), None, None
+        pos, *flat = ctx.saved_tensors
+        return ops.rope_axes(g, pos, list(zip(flat[::2], flat[1::2])), transpose=True), None, None
 
 
 def _f32_on(t: torch.Tensor, device: int, x: torch.Tensor) -> torch.Tensor:
@@ -219,7 +223,7 @@ def apply_rope_axes(x: torch.Tensor, positions: torch.Tensor, tables: Sequence[T
     x (B, N, D), or (B, N, H, D) with heads that share the angles.  ``tables``: per axis a (cos, sin) pair of
     (rows, s_a) tensors (see :func:`precompute_freqs_axes`); the axes' sections of 2 s_a channels follow one another, and
     inside a section channel k pairs with k + s_a, as :func:`apply_rope_2d` pairs its two halves; channels behind the
-    last section pass.  ``positions`` (N, A) for all samples, or (B, N, A).
+    last section pass.  ``positions`` (N, A) for all samples, or (B, N, A).  Only x has a gradient.
 
     ``validate``: an IndexError for a position outside its table, at the price of a synchronising read the first time a
     position tensor is seen.  Without it nothing is read back, and such a position makes its section of the token NaN."""
@@ -235,6 +239,8 @@ def apply_rope_axes(x: torch.Tensor, positions: torch.Tensor, tables: Sequence[T
         if len(shape) != 2 or shape != sin.shape or 0 in shape:
             raise ValueError(f"every table must be two (rows, pairs) tensors of one shape, got {tuple(shape)} and "
                              f"{tuple(sin.shape)}")
+        if (cos.requires_grad or sin.requires_grad) and torch.is_grad_enabled():
+            raise ValueError("the tables take no gradient: pass them detached")
         width += 2 * shape[1]
         tabs.append((_f32_on(cos, device, x), _f32_on(sin, device, x)))
     if width > D:

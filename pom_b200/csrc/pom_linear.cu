@@ -386,6 +386,8 @@ struct F32Plan {
   uint64_t b, scratch, total;
 };
 
+constexpr int64_t kF32Rows = 65535ll * 64;  // rows of one float32 product (a grid dimension of the FMA kernel)
+
 // A holds a_rows x a_cols values as it is stored, B b_rows x b_cols.
 F32Plan f32_plan(const pom_linear_args* a, int64_t M, int64_t N, int64_t K, int out_mode, int64_t a_rows, int64_t a_cols,
                  int64_t b_rows, int64_t b_cols) {
@@ -393,7 +395,7 @@ F32Plan f32_plan(const pom_linear_args* a, int64_t M, int64_t N, int64_t K, int 
   // Short sums run on the FMA kernel (see f32_planes_pay of the Python layer), and so do small products with sums of up to
   // 512 terms: one launch instead of three, which is what such a call waits for (500 x 300 -> 700 in training 139 us
   // against 174), while a longer chain would lose digits that a blocked sum keeps.
-  if (a->fma || K < 128 || (K <= 512 && static_cast<double>(M) * static_cast<double>(N) * static_cast<double>(K) < 0x1p27)) return p;
+  if (a->fma || M > kF32Rows || K < 128 || (K <= 512 && static_cast<double>(M) * static_cast<double>(N) * static_cast<double>(K) < 0x1p27)) return p;
   p.b = up256(pom_f32_planes_bytes(a_rows, a_cols));
   p.scratch = p.b + up256(pom_f32_planes_bytes(b_rows, b_cols));
   p.total = p.scratch + up256(pom_gemm_f32_planes_scratch(M, N, K, out_mode));
@@ -401,7 +403,17 @@ F32Plan f32_plan(const pom_linear_args* a, int64_t M, int64_t N, int64_t K, int 
 }
 
 int f32_product(const pom_gemm_args& g, const F32Plan& p, char* ws, int a_ready, int* status, cudaStream_t st) {
-  if (!p.total) return pom_gemm_f32(&g, st);
+  if (!p.total) {
+    pom_gemm_args part = g;
+    for (int64_t r = 0; r < g.M; r += kF32Rows) {  // more rows than one launch takes (K-major A: the rows of dx and y)
+      part.M = g.M - r < kF32Rows || g.a_mn_major ? g.M - r : kF32Rows;
+      part.A = static_cast<const float*>(g.A) + r * g.lda;
+      part.C = static_cast<float*>(g.C) + r * g.ldc;
+      const int rc = pom_gemm_f32(&part, st);
+      if (rc || g.a_mn_major) return rc;
+    }
+    return POM_OK;
+  }
   return pom_gemm_f32_planes(&g, ws, a_ready, ws + p.b, 0, ws + p.scratch, status, st);
 }
 

@@ -402,6 +402,18 @@ def test_rope_axes_positions_outside_the_tables():
         apply_rope_axes(x, p, tables)
 
 
+def test_rope_axes_notices_positions_that_change_before_backward():
+    tables = [(c.cuda(), s.cuda()) for c, s in precompute_freqs_axes((8, 8), (10, 12))]
+    x = rand(2, 5, 40, seed=6).requires_grad_(True)
+    pos = torch.randint(0, 9, (5, 2), device="cuda")
+    y = apply_rope_axes(x, pos, tables)
+    pos.add_(1)
+    with pytest.raises(RuntimeError, match="inplace"):
+        torch.autograd.grad(y.sum(), x)
+    with pytest.raises(ValueError, match="gradient"):
+        apply_rope_axes(x, pos, [(tables[0][0].clone().requires_grad_(True), tables[0][1]), tables[1]])
+
+
 # ---------------------------------------------------------------------------- all three: streams, graphs, repetition
 def block_pass(t):
     """The chain that a block runs, and all gradients."""
@@ -482,6 +494,28 @@ def test_same_bits_every_time_on_any_stream_and_from_graphs(dtype):
             for o in out:
                 o.zero_()
         torch.cuda.synchronize()
+
+
+def test_more_float32_rows_than_one_launch_takes():
+    M = 65535 * 64 + 70
+    x, w = rand(M, 8, seed=1), rand(8, 8, seed=2)
+    x.requires_grad_(True)
+    y = linear(x, w, activation="relu")
+    dx, = torch.autograd.grad(y, x, torch.ones_like(y))
+    with torch.no_grad():
+        for sl in (slice(0, 5), slice(M - 100, M), slice(65535 * 64 - 3, 65535 * 64 + 3)):
+            z = x[sl].double() @ w.double().t()
+            ze = 2 * 16 * E * (x[sl].double().abs() @ w.double().abs().t())
+            within(y[sl], z.clamp(min=0), ze, "y")
+            near = ((z.abs() <= ze).double()) @ w.double().abs()
+            within(dx[sl], (z > 0).double() @ w.double(), near + 32 * E * w.double().abs().sum(0), "dx")
+
+
+def test_vectors_and_keyword_arguments():
+    x, w, b, r, _ = linear_inputs(1, 64, 40, BF, seed=97)
+    y = linear(x=x[0], weight=w, bias=b, activation="silu", residual=r[0])
+    assert torch.equal(y, linear(x, w, b, activation="silu", residual=r)[0])
+    assert torch.equal(layer_norm(x=x[0], weight=x[0].abs()), layer_norm(x, x[0].abs())[0])
 
 
 def test_gradients_against_differences():
