@@ -96,7 +96,9 @@ def test_the_library_refuses_bad_arguments_before_it_launches():
     m.ldy, m.act = 8, 9
     assert L.pom_linear_fwd(ctypes.byref(m), None, None) == -4
     m.act, m.dtype, m.M, m.K, m.ldx, m.ldw = 0, 1, 1000, 256, 256, 256
-    assert L.pom_linear_fwd_workspace(ctypes.byref(m)) >= 6 * (1000 * 256 + 8 * 256)
+    assert L.pom_linear_fwd_workspace(ctypes.byref(m)) == 0  # a small product: the FMA kernel
+    m.K = m.ldx = m.ldw = 1024
+    assert L.pom_linear_fwd_workspace(ctypes.byref(m)) >= 6 * (1000 * 1024 + 8 * 1024)
     assert L.pom_linear_fwd(ctypes.byref(m), None, None) == -8  # float32 operands without room for their planes
     m.fma = 1
     assert L.pom_linear_fwd_workspace(ctypes.byref(m)) == 0
