@@ -354,6 +354,11 @@ def stream_ptr() -> int:
     return torch.cuda.current_stream().cuda_stream
 
 
+def stream_of(index: int) -> int:
+    """As :func:`stream_ptr`, for the current device when its index is known already."""
+    return _raw_stream(index) if _raw_stream is not None else torch.cuda.current_stream(index).cuda_stream
+
+
 def ptr(t) -> int | None:
     return None if t is None else t.data_ptr()
 

@@ -959,8 +959,8 @@ def rows_of(t: torch.Tensor, align: bool = False):
     return t, ld
 
 
-def _same_device(x: torch.Tensor, *others) -> None:
-    """All tensors on x's GPU (others may be None)."""
+def _same_device(x: torch.Tensor, *others) -> int:
+    """The index of x's GPU, on which all others (which may be None) must live."""
     i = x.get_device()
     if i < 0:
         raise RuntimeError("pom_b200 runs on CUDA tensors only (no CPU fallback)")
@@ -969,6 +969,7 @@ def _same_device(x: torch.Tensor, *others) -> None:
             if t.get_device() < 0:
                 raise RuntimeError("pom_b200 runs on CUDA tensors only (no CPU fallback)")
             raise RuntimeError("all tensors of one call must live on the same GPU")
+    return i
 
 
 _DTYPE = {torch.bfloat16: _abi.POM_BF16, torch.float32: _abi.POM_F32}
@@ -978,11 +979,11 @@ def layer_norm_fwd(x: torch.Tensor, weight: Optional[torch.Tensor], bias: Option
                    want_stats: bool):
     """Layer norm over the last dimension: (y, stats), stats (M, 2) fp32 = mean and 1 / sqrt(var + eps) of every row, or
     None.  ``weight`` and ``bias`` contiguous, of one dtype."""
-    _same_device(x, weight, bias)
+    dev = _same_device(x, weight, bias)
     x, ld = rows_of(x)
     D = x.shape[-1]
     M = x.numel() // D
-    y = torch.empty_like(x, memory_format=torch.contiguous_format)
+    y = torch.empty_like(x) if ld == D else x.new_empty(x.shape)
     stats = x.new_empty((M, 2), dtype=torch.float32) if want_stats else None
     if M:
         a = LayerNormArgs()
@@ -994,19 +995,19 @@ def layer_norm_fwd(x: torch.Tensor, weight: Optional[torch.Tensor], bias: Option
                 a.bias = bias.data_ptr()
         if stats is not None:
             a.stats = stats.data_ptr()
-        _abi.check(_abi.lib().pom_layer_norm_fwd(C.byref(a), _abi.stream_ptr()), "pom_layer_norm_fwd")
+        _abi.check(_abi.lib().pom_layer_norm_fwd(C.byref(a), _abi.stream_of(dev)), "pom_layer_norm_fwd")
     return y, stats
 
 
 def layer_norm_bwd(dy: torch.Tensor, x: torch.Tensor, weight: Optional[torch.Tensor], stats: torch.Tensor, *,
                    want_dx: bool, want_dw: bool, want_db: bool):
     """(dx, dweight, dbias) of :func:`layer_norm_fwd`; what is not wanted is None."""
-    _same_device(dy, x, weight, stats)
+    dev = _same_device(dy, x, weight, stats)
     x, ldx = rows_of(x)
     dy, ldg = rows_of(dy)
     D = x.shape[-1]
     M = x.numel() // D
-    dx = torch.empty_like(x, memory_format=torch.contiguous_format) if want_dx else None
+    dx = (torch.empty_like(x) if ldx == D else x.new_empty(x.shape)) if want_dx else None
     dw = torch.empty_like(weight) if want_dw else None
     db = torch.empty_like(weight) if want_db else None
     if M == 0:
@@ -1027,7 +1028,7 @@ def layer_norm_bwd(dy: torch.Tensor, x: torch.Tensor, weight: Optional[torch.Ten
         if dw is not None or db is not None:
             ws = stats.new_empty(L.pom_layer_norm_bwd_workspace(C.byref(a)) // 4)
             a.workspace = ws.data_ptr()
-    _abi.check(L.pom_layer_norm_bwd(C.byref(a), _abi.stream_ptr()), "pom_layer_norm_bwd")
+    _abi.check(L.pom_layer_norm_bwd(C.byref(a), _abi.stream_of(dev)), "pom_layer_norm_bwd")
     return dx, dw, db
 
 
@@ -1062,7 +1063,7 @@ def linear_fwd(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor], a
                residual: Optional[torch.Tensor], want_z: bool):
     """act(z) + residual with z = x·wᵀ + bias: (y, z), z (M, N) in x's dtype or None.  x (..., K), w (N, K), both bf16
     (K and N multiples of 8) or both float32; ``bias`` contiguous, bf16 or float32."""
-    _same_device(x, w, bias, residual)
+    dev = _same_device(x, w, bias, residual)
     bf16 = x.dtype == torch.bfloat16
     x, ldx = rows_of(x, bf16)
     w, ldw = rows_of(w, bf16)
@@ -1084,20 +1085,20 @@ def linear_fwd(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor], a
     L = _abi.lib()
     if not bf16:
         ws = _linear_workspace(L.pom_linear_fwd_workspace, a, x)  # noqa: F841 (alive until the call below)
-    _abi.check(L.pom_linear_fwd(C.byref(a), _abi.status_ptr(x.get_device()), _abi.stream_ptr()), "pom_linear_fwd")
+    _abi.check(L.pom_linear_fwd(C.byref(a), _abi.status_ptr(dev), _abi.stream_of(dev)), "pom_linear_fwd")
     return y, z
 
 
 def linear_bwd(dy: torch.Tensor, x: torch.Tensor, w: torch.Tensor, act: Optional[str], z: Optional[torch.Tensor], *,
                want_dx: bool, want_dw: bool, bias_dtype: Optional[torch.dtype]):
     """(dx, dw, dbias) of :func:`linear_fwd` (dbias where ``bias_dtype`` is given); what is not wanted is None."""
-    _same_device(dy, x, w, z)
+    dev = _same_device(dy, x, w, z)
     bf16 = x.dtype == torch.bfloat16
     x, ldx = rows_of(x, bf16)
     w, ldw = rows_of(w, bf16)
     N, K = w.shape
     M = x.numel() // K
-    dx = torch.empty_like(x, memory_format=torch.contiguous_format) if want_dx else None
+    dx = (torch.empty_like(x) if ldx == K else x.new_empty(x.shape)) if want_dx else None
     dw = w.new_empty((N, K)) if want_dw else None
     db = w.new_empty(N, dtype=bias_dtype) if bias_dtype is not None else None
     if M == 0:
@@ -1115,14 +1116,14 @@ def linear_bwd(dy: torch.Tensor, x: torch.Tensor, w: torch.Tensor, act: Optional
         a.dw = dw.data_ptr()
     L = _abi.lib()
     ws = _linear_workspace(L.pom_linear_bwd_workspace, a, x)  # noqa: F841 (alive until the call below)
-    _abi.check(L.pom_linear_bwd(C.byref(a), _abi.status_ptr(x.get_device()), _abi.stream_ptr()), "pom_linear_bwd")
+    _abi.check(L.pom_linear_bwd(C.byref(a), _abi.status_ptr(dev), _abi.stream_of(dev)), "pom_linear_bwd")
     return dx, dw, db
 
 
 def rope_axes(x: torch.Tensor, pos: torch.Tensor, tables, transpose: bool = False) -> torch.Tensor:
     """Rotation of x (B, N, D) or (B, N, H, D) by positions of several axes (``pom_rope_axes``).  pos (N, A) or (B, N, A)
     int64 contiguous; ``tables``: one (cos, sin) pair of contiguous fp32 (rows, pairs) tensors per axis."""
-    _same_device(x, pos)
+    dev = _same_device(x, pos)
     stride, shape = x.stride(), x.shape
     if stride[-1] != 1 and shape[-1] > 1:
         x = x.contiguous()
@@ -1156,7 +1157,7 @@ def rope_axes(x: torch.Tensor, pos: torch.Tensor, tables, transpose: bool = Fals
         if shape[2] > 1:
             a.xs_h = stride[2]
     a.axes, a.dtype, a.pos_per_sample, a.transpose = axes, _DTYPE[x.dtype], pos.dim() == 3, transpose
-    _abi.check(_abi.lib().pom_rope_axes(C.byref(a), _abi.stream_ptr()), "pom_rope_axes")
+    _abi.check(_abi.lib().pom_rope_axes(C.byref(a), _abi.stream_of(dev)), "pom_rope_axes")
     return y
 
 
