@@ -10,22 +10,23 @@
 
 namespace pomk {
 
-template <int ACT>
-__device__ __forceinline__ void linear_act32(float (&v)[32]) {
+template <int ACT, int LEN>
+__device__ __forceinline__ void linear_act_row(float (&v)[LEN]) {
 #pragma unroll
-  for (int i = 0; i < 32; i += 2) {
+  for (int i = 0; i < LEN; i += 2) {
     const F2 y = linear_act2<true>(ACT, F2(v[i], v[i + 1]));
     v[i] = y.v.x, v[i + 1] = y.v.y;
   }
 }
 
-// 32 values of a row; the choice of the activation stands outside their loop.
-__device__ __forceinline__ void linear_act32(int act, float (&v)[32]) {
+// Adjacent values of a row; the choice of the activation stands outside their loop.
+template <int LEN>
+__device__ __forceinline__ void linear_act_row(int act, float (&v)[LEN]) {
   switch (act) {
-    case POM_ACT_GELU: linear_act32<POM_ACT_GELU>(v); break;
-    case POM_ACT_GELU_TANH: linear_act32<POM_ACT_GELU_TANH>(v); break;
-    case POM_ACT_SILU: linear_act32<POM_ACT_SILU>(v); break;
-    case POM_ACT_RELU: linear_act32<POM_ACT_RELU>(v); break;
+    case POM_ACT_GELU: linear_act_row<POM_ACT_GELU>(v); break;
+    case POM_ACT_GELU_TANH: linear_act_row<POM_ACT_GELU_TANH>(v); break;
+    case POM_ACT_SILU: linear_act_row<POM_ACT_SILU>(v); break;
+    case POM_ACT_RELU: linear_act_row<POM_ACT_RELU>(v); break;
     default: break;
   }
 }
@@ -102,7 +103,7 @@ struct EpiLinear {
         pack32(v, pk);
         if (t.rows_valid > 0) store_block<1>(RES ? base + 4096 : base, &maps.out0, pk, lane, col, y, t.b);
       }
-      linear_act32(p.act, v);
+      linear_act_row(p.act, v);
       if constexpr (RES) {
         float r[32];
         if (alive) alive = mbar_wait(io.bar, io.load_phase, io.abort_flag, io.status, kStatusEpilogueTimeout);

@@ -354,7 +354,7 @@ gemm_tcgen05_2cta_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_c
         if constexpr (Epi::kStager) mbar_arrive(&sm.sempty_bar[acc]);
       }
     }
-    if (lane == 0) bulk_wait_all();
+    if (lane == 0) bulk_wait_read<0>();
   } else {
     // ------------------------------------------------------------ stager (both CTAs, own rows)
     if constexpr (Epi::kStager) {

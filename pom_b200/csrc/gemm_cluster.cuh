@@ -6,8 +6,8 @@
 // while a few of them read.  A cluster of `size` CTAs divides that time by `size`.  Every CTA owns BN / size columns of the
 // result: it sends the other columns of its partial tile to their owners (st.shared::cluster, 512 adjacent bytes a warp: with
 // the rows apart, the same stores took 4 us instead of 1), and after one cluster barrier adds what it has received to its own
-// accumulator, in the order of the ranks: the same bits on every run.  Then bias, activation and residual, from
-// registers to global memory; bias and residual are fetched while the main loop runs.
+// accumulator, in the order of the ranks: the same bits on every run.  Then bias, activation and residual, which
+// were fetched while the main loop ran, and bulk stores of 32 x 32 blocks (16 columns: from registers).
 //
 // Roles and waits as in gemm_sm100.cuh: warp 0 loads, warp 1 issues the MMAs, warps 2 to 9 are the epilogue; every wait on
 // a barrier in shared memory is bounded, and every thread reaches both cluster barriers whatever happened before.
@@ -49,7 +49,8 @@ __device__ __forceinline__ uint32_t recv_offset(int row, int j) { return static_
 
 template <int BN, bool A_MN, bool B_MN>
 __global__ void __launch_bounds__(kClusterThreads, 1)
-gemm_cluster_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const ClusterDev a,
+gemm_cluster_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
+                    const __grid_constant__ CUtensorMap tmY, const __grid_constant__ CUtensorMap tmZ, const ClusterDev a,
                     int* __restrict__ status) {
   using S = ClusterSmem<BN>;
   constexpr int kABytes = kBM * kBK * 2;
@@ -156,10 +157,16 @@ gemm_cluster_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
   const int quarter = warp & 3, half = (warp - 2) >> 2;  // epilogue warps: TMEM lanes of this warp, and which pieces
   const int row = quarter * 32 + lane;
   const uint32_t acc = tmem + (static_cast<uint32_t>(quarter * 32) << 16);
-  constexpr int kOwn = 128 / 16 / 2;  // most pieces of 16 columns that a warp finishes
   const long long r = row0 + row;
   const int first = col0 + static_cast<int>(rank) * slice;  // first column that this CTA finishes
-  uint4 res[kOwn][2];
+  const int width = slice < 32 ? slice : 32;                 // columns of a chunk; a warp takes chunks half, half + 2, ...
+  // residual of the eight columns at `at` of this CTA's slice (N is a multiple of 8)
+  auto residual = [&](int at) {
+    if (a.residual && r < a.M && at < slice && first + at < a.N)
+      return __ldg(reinterpret_cast<const uint4*>(a.residual + r * a.ldr + first + at));
+    return make_uint4(0, 0, 0, 0);
+  };
+  uint4 res = make_uint4(0, 0, 0, 0);
   if (warp >= 2) {
     const int e = threadIdx.x - 64;
     if (e < slice) {
@@ -169,15 +176,7 @@ gemm_cluster_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
                        : __bfloat162float(__ldg(static_cast<const __nv_bfloat16*>(a.bias) + first + e));
       bias_sm[e] = b;
     }
-#pragma unroll
-    for (int i = 0; i < kOwn; ++i)
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int p = half + 2 * i, c = first + p * 16 + 8 * h;  // N is a multiple of 8
-        res[i][h] = make_uint4(0, 0, 0, 0);
-        if (a.residual && r < a.M && p * 16 < slice && c < a.N)
-          res[i][h] = __ldg(reinterpret_cast<const uint4*>(a.residual + r * a.ldr + c));
-      }
+    res = residual(half * width);
     ok = mbar_wait(done_bar, 0, abort_flag, status, kStatusEpilogueTimeout);
     ok = __all_sync(0xffffffffu, ok);
     tc_fence_after();
@@ -210,66 +209,64 @@ gemm_cluster_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
   __syncwarp();
   cluster_sync_all();  // every partial tile has arrived; nobody writes to another CTA after this
   if (warp >= 2 && ok) {
+    uint8_t* buf = tiles + (warp - 2) * 8192;  // the operand tiles have been read: two blocks for each of this warp's chunks
+    const int top = row0 + quarter * 32;
+#pragma unroll 1
+    for (int at0 = half * width; at0 < slice && first + at0 < a.N; at0 += 2 * width, buf += 4096) {  // warp-uniform
+#pragma unroll 1
+      for (int j = 0; j < width / 8; ++j) {
+        const int at = at0 + 8 * j;
+        float own[8], v[8];
+        tmem_ld8(acc + rank * slice + at, own);
+        const uint4 mine = res;
+        res = residual(j + 1 < width / 8 ? at + 8 : at0 + 2 * width);  // of the columns after these
+        tmem_ld_wait();
 #pragma unroll
-    for (int i = 0; i < kOwn; ++i) {
-      const int p = half + 2 * i, col = first + p * 16;
-      if (p * 16 >= slice || col >= a.N) break;  // warp-uniform
-      float own[16], v[16];
-      tmem_ld16<0>(acc + rank * slice + p * 16, own);
-      tmem_ld_wait();
-#pragma unroll
-      for (int k = 0; k < 16; ++k) v[k] = 0.f;
-      for (uint32_t s = 0; s < size; ++s) {
-        if (s == rank) {
-#pragma unroll
-          for (int k = 0; k < 16; ++k) v[k] += own[k];
-        } else {
+        for (int k = 0; k < 8; ++k) v[k] = 0.f;
+        for (uint32_t s = 0; s < size; ++s) {
           const uint8_t* src = recv + (s < rank ? s : s - 1) * (kBM * slice * 4);
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const float4 q = *reinterpret_cast<const float4*>(src + recv_offset(row, p * 4 + j));
-            v[4 * j] += q.x, v[4 * j + 1] += q.y, v[4 * j + 2] += q.z, v[4 * j + 3] += q.w;
+          float4 p = make_float4(own[0], own[1], own[2], own[3]), q = make_float4(own[4], own[5], own[6], own[7]);
+          if (s != rank) {
+            p = *reinterpret_cast<const float4*>(src + recv_offset(row, at / 4));
+            q = *reinterpret_cast<const float4*>(src + recv_offset(row, at / 4 + 1));
           }
+          v[0] += p.x, v[1] += p.y, v[2] += p.z, v[3] += p.w;
+          v[4] += q.x, v[5] += q.y, v[6] += q.z, v[7] += q.w;
+        }
+#pragma unroll
+        for (int k = 0; k < 8; k += 4) {
+          const float4 b = *reinterpret_cast<const float4*>(bias_sm + at + k);
+          v[k] += b.x, v[k + 1] += b.y, v[k + 2] += b.z, v[k + 3] += b.w;
+        }
+        const uint4 pz = make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]));
+        linear_act_row(a.act, v);
+        const uint32_t w[4] = {mine.x, mine.y, mine.z, mine.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          v[2 * e] += __uint_as_float(w[e] << 16);
+          v[2 * e + 1] += __uint_as_float(w[e] & 0xffff0000u);
+        }
+        const uint4 py = make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]));
+        if (width == 32) {
+          *reinterpret_cast<uint4*>(buf + swz64(lane, j)) = py;
+          if (a.z) *reinterpret_cast<uint4*>(buf + 2048 + swz64(lane, j)) = pz;
+        } else if (r < a.M && first + at < a.N) {
+          *reinterpret_cast<uint4*>(a.y + r * a.ldy + first + at) = py;
+          if (a.z) *reinterpret_cast<uint4*>(a.z + r * a.N + first + at) = pz;
+        }
+        __syncwarp();  // the next tensor-memory load wants the whole warp
+      }
+      if (width == 32 && top < a.M) {  // blocks are clipped at the last row and column
+        fence_async_smem();
+        __syncwarp();
+        if (lane == 0) {
+          tma_store_3d(&tmY, buf, first + at0, top, 0);
+          if (a.z) tma_store_3d(&tmZ, buf + 2048, first + at0, top, 0);
+          bulk_commit();
         }
       }
-#pragma unroll
-      for (int k = 0; k < 16; k += 4) {
-        const float4 b = *reinterpret_cast<const float4*>(bias_sm + p * 16 + k);
-        v[k] += b.x, v[k + 1] += b.y, v[k + 2] += b.z, v[k + 3] += b.w;
-      }
-      if (a.z && r < a.M) {
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-          if (col + 8 * h < a.N) {
-            const float* t = v + 8 * h;
-            *reinterpret_cast<uint4*>(a.z + r * a.N + col + 8 * h) =
-                make_uint4(pack_bf16x2(t[0], t[1]), pack_bf16x2(t[2], t[3]), pack_bf16x2(t[4], t[5]), pack_bf16x2(t[6], t[7]));
-          }
-      }
-#pragma unroll
-      for (int k = 0; k < 16; k += 2) {
-        const F2 y = linear_act2<true>(a.act, F2(v[k], v[k + 1]));
-        v[k] = y.v.x, v[k + 1] = y.v.y;
-      }
-      if (r < a.M) {
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const int c = col + 8 * h;
-          if (c < a.N) {
-            float* u = v + 8 * h;
-            const uint32_t w[4] = {res[i][h].x, res[i][h].y, res[i][h].z, res[i][h].w};
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              u[2 * e] += __uint_as_float(w[e] << 16);
-              u[2 * e + 1] += __uint_as_float(w[e] & 0xffff0000u);
-            }
-            *reinterpret_cast<uint4*>(a.y + r * a.ldy + c) =
-                make_uint4(pack_bf16x2(u[0], u[1]), pack_bf16x2(u[2], u[3]), pack_bf16x2(u[4], u[5]), pack_bf16x2(u[6], u[7]));
-          }
-        }
-      }
-      __syncwarp();  // the next piece's tensor-memory load wants the whole warp
     }
+    if (lane == 0) bulk_wait_read<0>();  // the stores have read their blocks; the grid's end waits for the rest
   }
   tc_fence_before();
   __syncthreads();
@@ -313,14 +310,15 @@ inline int max_clusters(int size) {
   return n;
 }
 
-// Estimated time in microseconds, launch apart: per wave of CTAs the k-blocks of one rank (0.285 each with 128 columns, 0.37
-// with 256, where the L2 delivers: 12 TB/s) and the exchange, against the same product by whole tiles.
+// Estimated time in microseconds, launch apart: per wave of CTAs the k-blocks of one rank (0.285 each with 128 columns; 0.46 with
+// 256, for which only three stages fit) and the exchange, which grows with the columns that a CTA finishes, against the same
+// product by whole tiles.
 inline ClusterPlan pick_cluster(int64_t M, int64_t N, int64_t K) {
   const int64_t kb = ceil_div(K, kBK), mt = ceil_div(M, kBM);
   const int sms = sm_count();
   // k-blocks of CTAs that take `bytes` each: bound by the SM's own intake, or by what the L2 gives all of them
   auto block_us = [](int64_t ctas, double alone, double bytes) {
-    const double shared = static_cast<double>(ctas) * bytes / 12.3e6;
+    const double shared = static_cast<double>(ctas) * bytes / 13.5e6;
     return shared > alone ? shared : alone;
   };
   struct Whole {
@@ -335,25 +333,28 @@ inline ClusterPlan pick_cluster(int64_t M, int64_t N, int64_t K) {
     const double t = ceil_div(units, w.slots) * (kb * block_us(at_once * w.ctas, w.alone, w.bytes) + 1.0);
     if (best < 0 || t < best) best = t;
   }
-  best *= 0.93;  // an estimate this close is not worth the exchange
+  best *= 0.97;  // an estimate this close is not worth the exchange
   ClusterPlan p{128, 1};
   for (int bn = 128; bn <= 256; bn += 128)
     for (int size = 2; size <= (bn == 128 ? kClusterMax : 2); size *= 2) {
       if (kb < 2 * size) continue;
       const int64_t units = mt * ceil_div(N, bn), slots = max_clusters(size), at_once = (units < slots ? units : slots) * size;
-      const double block = bn == 128 ? block_us(at_once, 0.285, 32768.0) : block_us(at_once, 0.37, 49152.0);
-      const double t = ceil_div(units, slots) * (ceil_div(kb, size) * block + 2.0);
+      const double block = bn == 128 ? block_us(at_once, 0.285, 32768.0) : block_us(at_once, 0.46, 49152.0);
+      const double t = ceil_div(units, slots) * (ceil_div(kb, size) * block + 1.5 + 0.024 * (bn / size));
       if (t < best) best = t, p = ClusterPlan{bn, size};
     }
   return p;
 }
 
-template <int BN, bool A_MN, bool B_MN>
+template <int BN, bool B_MN>
 int launch_cluster(const Operands& o, int size, ClusterDev d, int* status, cudaStream_t st) {
-  CUtensorMap tmA, tmB;
+  CUtensorMap tmA, tmB, tmY, tmZ;
   int rc = build_maps(o, BN, &tmA, &tmB);
   if (rc) return rc;
-  auto kern = gemm_cluster_kernel<BN, A_MN, B_MN>;
+  if ((rc = make_io_map(&tmY, d.y, o.N, o.M, 1, d.ldy))) return rc;
+  tmZ = tmY;  // unused without z
+  if (d.z && (rc = make_io_map(&tmZ, d.z, o.N, o.M, 1, o.N))) return rc;
+  auto kern = gemm_cluster_kernel<BN, false, B_MN>;
   constexpr int smem = ClusterSmem<BN>::kBytes;
   static_assert(smem <= 232448, "more shared memory than a CTA may have");
   static std::atomic<uint64_t> attr_set{0};
@@ -373,7 +374,7 @@ int launch_cluster(const Operands& o, int size, ClusterDev d, int* status, cudaS
   attr[1].val.clusterDim.x = size, attr[1].val.clusterDim.y = 1, attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 2;
-  if (cudaLaunchKernelEx(&cfg, kern, tmA, tmB, d, status) != cudaSuccess) {
+  if (cudaLaunchKernelEx(&cfg, kern, tmA, tmB, tmY, tmZ, d, status) != cudaSuccess) {
     (void)cudaGetLastError();
     return POM_ERR_CUDA;
   }
@@ -386,10 +387,8 @@ inline int cluster_product(const Operands& o, const ClusterPlan& p, const Cluste
   const int rc = check_operands(o);
   if (rc) return rc;
   if (o.b_mn)
-    return p.bn == 128 ? launch_cluster<128, false, true>(o, p.size, d, status, st)
-                       : launch_cluster<256, false, true>(o, p.size, d, status, st);
-  return p.bn == 128 ? launch_cluster<128, false, false>(o, p.size, d, status, st)
-                     : launch_cluster<256, false, false>(o, p.size, d, status, st);
+    return p.bn == 128 ? launch_cluster<128, true>(o, p.size, d, status, st) : launch_cluster<256, true>(o, p.size, d, status, st);
+  return p.bn == 128 ? launch_cluster<128, false>(o, p.size, d, status, st) : launch_cluster<256, false>(o, p.size, d, status, st);
 }
 
 }  // namespace pomh

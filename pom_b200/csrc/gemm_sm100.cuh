@@ -525,7 +525,7 @@ gemm_tcgen05_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
         if constexpr (Epi::kStager) mbar_arrive(&sm.sempty_bar[acc]);
       }
     }
-    if (lane == 0) bulk_wait_all();  // bulk stores still reading this warp's staging block
+    if (lane == 0) bulk_wait_read<0>();  // bulk stores still reading this warp's staging block; the grid's end waits for the rest
   } else {
     // ------------------------------------------------------------ stager
     if constexpr (Epi::kStager) {

@@ -224,7 +224,8 @@ def test_linear_sizes(M, K, N, dtype):
 
 @pytest.mark.parametrize("act", [None, "gelu", "relu"])
 @pytest.mark.parametrize("M, K, N", [(65, 1096, 136), (130, 2056, 264), (300, 1160, 1096), (1000, 136, 72), (2049, 72, 136),
-                                     (200, 1000, 1160), (500, 2312, 520), (1100, 2120, 1032), (2000, 4104, 1000), (129, 264, 120)])
+                                     (200, 1000, 1160), (500, 2312, 520), (1100, 2120, 1032), (2000, 4104, 1000), (129, 264, 120),
+                                     (1000, 3080, 1160), (385, 4616, 264), (513, 1032, 2056)])
 def test_linear_products_cut_along_their_sum(M, K, N, act):
     """Few output tiles and a long sum: the product and the data gradient run on clusters of two to eight blocks, the
     weight gradient in slabs."""
