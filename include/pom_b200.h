@@ -714,8 +714,12 @@ typedef struct pom_rope_axes_args {
   int32_t pos_per_sample, transpose;
 } pom_rope_axes_args;
 int pom_rope_axes(const pom_rope_axes_args* a, void* stream);
-/* Smallest and largest value of every column of the (rows, axes) positions: info[2 a], info[2 a + 1]. */
-int pom_pos_range(const int64_t* pos, int64_t rows, int32_t axes, int64_t* info, void* stream);
+#define POM_POS_RANGE_BLOCKS 16
+/* Range of every column of the (rows, axes) positions, into page-locked host memory that the device can address, valid once
+ * the stream has got there: the first pom_pos_range_blocks(rows) rows of host_info (POM_POS_RANGE_BLOCKS, 2 * axes) hold
+ * the smallest (2 a) and largest (2 a + 1) positions of as many parts of the rows. */
+int32_t pom_pos_range_blocks(int64_t rows);
+int pom_pos_range(const int64_t* pos, int64_t rows, int32_t axes, int64_t* host_info, void* stream);
 
 /* Asynchronous device-to-device copy of `bytes` bytes on the stream (cudaMemcpyAsync; no kernel). */
 int pom_copy_bytes(void* dst, const void* src, int64_t bytes, void* stream);

@@ -207,6 +207,7 @@ class LinearArgs(C.Structure):
 
 
 ROPE_MAX_AXES = 4
+POS_RANGE_BLOCKS = 16
 
 
 class RopeAxesArgs(C.Structure):  # the C arrays cos, sin, len and pairs as single fields, which are cheaper to set
@@ -307,6 +308,7 @@ _SIGNATURES = {
     "pom_linear_bwd_workspace": (C.c_uint64, [C.POINTER(LinearArgs)]),
     "pom_linear_bwd": (C.c_int, [C.POINTER(LinearArgs), C.c_void_p, C.c_void_p]),
     "pom_rope_axes": (C.c_int, [C.POINTER(RopeAxesArgs), C.c_void_p]),
+    "pom_pos_range_blocks": (C.c_int32, [C.c_int64]),
     "pom_pos_range": (C.c_int, [C.c_void_p, C.c_int64, C.c_int32, C.c_void_p, C.c_void_p]),
     "pom_copy_bytes": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int64, C.c_void_p]),
 }

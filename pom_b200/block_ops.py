@@ -225,8 +225,8 @@ def apply_rope_axes(x: torch.Tensor, positions: torch.Tensor, tables: Sequence[T
     inside a section channel k pairs with k + s_a, as :func:`apply_rope_2d` pairs its two halves; channels behind the
     last section pass.  ``positions`` (N, A) for all samples, or (B, N, A).  Only x has a gradient.
 
-    ``validate``: an IndexError for a position outside its table, at the price of a synchronising read the first time a
-    position tensor is seen.  Without it nothing is read back, and such a position makes its section of the token NaN."""
+    ``validate``: an IndexError for a position outside its table, for which the call waits until the stream has come
+    to it (and cannot be captured).  Without it nothing is read back, and such a position makes its section of the token NaN."""
     _check_tokens(x)
     if x.dim() not in (3, 4):
         raise ValueError(f"expected a (B, N, D) or (B, N, H, D) tensor, got {tuple(x.shape)}")
@@ -253,15 +253,17 @@ def apply_rope_axes(x: torch.Tensor, positions: torch.Tensor, tables: Sequence[T
         if pos.dtype.is_floating_point or pos.dtype == torch.bool or pos.dtype.is_complex:
             raise TypeError(f"positions must be integers, got {pos.dtype}")
         pos = pos.to(device=x.device, dtype=torch.int64)
-    if validate and pos.numel():
-        for a, ((lo, hi), (cos, _)) in enumerate(zip(ops.pos_range(pos), tabs)):
-            if lo < 0 or hi >= cos.shape[0]:
-                raise IndexError(f"positions of axis {a} span [{lo}, {hi}] but its table has {cos.shape[0]} rows")
     if not pos.is_contiguous():
         pos = pos.contiguous()
-    if x.requires_grad and torch.is_grad_enabled():
-        return _RotateAxes.apply(x, pos, tabs)
-    return ops.rope_axes(x, pos, tabs)
+    validate = validate and pos.numel() > 0
+    if validate:  # the rotation follows at once (a bad position is harmless there); only the answer is waited for
+        ops.pos_range_start(pos)
+    y = _RotateAxes.apply(x, pos, tabs) if x.requires_grad and torch.is_grad_enabled() else ops.rope_axes(x, pos, tabs)
+    if validate:
+        for a, ((lo, hi), (cos, _)) in enumerate(zip(ops.pos_range_wait(pos), tabs)):
+            if lo < 0 or hi >= cos.shape[0]:
+                raise IndexError(f"positions of axis {a} span [{lo}, {hi}] but its table has {cos.shape[0]} rows")
+    return y
 
 
 def precompute_freqs_axes(pairs: Sequence[int], rows: Sequence[int], base: float = 10000.0):

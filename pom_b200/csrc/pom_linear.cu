@@ -426,7 +426,7 @@ struct BwdPlan {
 BwdPlan bwd_plan(const pom_linear_args* a) {
   BwdPlan p{};
   const int per = a->dtype == POM_BF16 ? 8 : 4;
-  p.vec = a->N % per || a->ld_dy % per || !aligned16(a->dy) ? 1 : per;
+  p.vec = a->N % per || a->ld_dy % per || !aligned16(a->dy) || !aligned16(a->z) ? 1 : per;
   p.chunk = dz_chunk(a->M, a->N, p.vec, a->act == POM_ACT_NONE);
   p.chunks = static_cast<int>(ceil_div(a->M, p.chunk));
   const bool bf16 = a->dtype == POM_BF16;
@@ -575,6 +575,7 @@ int pom_linear_bwd(const pom_linear_args* a, int* status, void* stream) {
   const BwdPlan p = bwd_plan(a);
   if (p.total && !a->workspace) return POM_ERR_NULL;
   if (!aligned16(a->workspace) || !aligned16(a->dz)) return POM_ERR_BAD_ALIGN;
+  if (a->dtype == POM_BF16 && (!aligned16(a->dw) || !aligned16(a->dx))) return POM_ERR_BAD_ALIGN;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   char* ws = static_cast<char*>(a->workspace);
   void* own_dz = a->dz ? a->dz : ws + p.dz;

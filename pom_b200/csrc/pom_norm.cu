@@ -575,6 +575,7 @@ int check_norm(const pom_layer_norm_args* a) {
   if (a->wdtype != POM_F32 && (a->wdtype != POM_BF16 || a->dtype != POM_BF16)) return POM_ERR_UNSUPPORTED;
   if (a->bias && !a->weight) return POM_ERR_UNSUPPORTED;
   if (a->ldx < a->D) return POM_ERR_BAD_STRIDE;
+  if (reinterpret_cast<uintptr_t>(a->stats) & 7u) return POM_ERR_BAD_ALIGN;
   return POM_OK;
 }
 
@@ -632,6 +633,7 @@ int pom_layer_norm_bwd(const pom_layer_norm_args* a, void* stream) {
   if (!a->dy || !a->stats || (grads && !a->workspace)) return POM_ERR_NULL;
   if (!a->dx && !grads) return POM_OK;
   if (a->ld_dy < a->D || (a->dx && a->ld_dx < a->D)) return POM_ERR_BAD_STRIDE;
+  if (!aligned16(a->workspace)) return POM_ERR_BAD_ALIGN;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const NormPlan p = bwd_plan(a);
   NormDev d = norm_dev(a);

@@ -110,33 +110,40 @@ __global__ void __launch_bounds__(kThreads) rope_axes_kernel(const AxesDev a) {
   }
 }
 
-// Smallest and largest position per axis: info[2 * axis] and info[2 * axis + 1].  One block.
+// Smallest and largest position per axis of the block's rows, written side by side to the host's memory.
 __global__ void __launch_bounds__(1024) pos_range_kernel(const long long* __restrict__ pos, long long rows, int axes,
-                                                         long long* __restrict__ info) {
-  __shared__ long long s_lo[32], s_hi[32];
+                                                         long long* host_info) {
+  __shared__ long long sm[2 * kMaxAxes][32];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  for (int c = 0; c < axes; ++c) {
-    long long lo = LLONG_MAX, hi = LLONG_MIN;
-    for (long long i = threadIdx.x; i < rows; i += 1024) {
-      const long long p = __ldg(pos + i * axes + c);
-      lo = p < lo ? p : lo;
-      hi = p > hi ? p : hi;
-    }
-    for (int o = 16; o; o >>= 1) {
-      const long long l = __shfl_xor_sync(0xffffffffu, lo, o), h = __shfl_xor_sync(0xffffffffu, hi, o);
-      lo = l < lo ? l : lo;
-      hi = h > hi ? h : hi;
-    }
-    if (lane == 0) s_lo[warp] = lo, s_hi[warp] = hi;
-    __syncthreads();
-    if (threadIdx.x == 0) {
-      for (int w = 1; w < 32; ++w) {
-        lo = s_lo[w] < lo ? s_lo[w] : lo;
-        hi = s_hi[w] > hi ? s_hi[w] : hi;
+  long long hi[kMaxAxes], lo[kMaxAxes];
+#pragma unroll
+  for (int c = 0; c < kMaxAxes; ++c) hi[c] = LLONG_MIN, lo[c] = LLONG_MAX;
+#pragma unroll 4
+  for (long long i = blockIdx.x * 1024ll + threadIdx.x; i < rows; i += gridDim.x * 1024ll)
+#pragma unroll
+    for (int c = 0; c < kMaxAxes; ++c)
+      if (c < axes) {
+        const long long p = __ldg(pos + i * axes + c);
+        hi[c] = p > hi[c] ? p : hi[c];
+        lo[c] = p < lo[c] ? p : lo[c];
       }
-      info[2 * c] = lo, info[2 * c + 1] = hi;
+#pragma unroll
+  for (int c = 0; c < kMaxAxes; ++c) {
+    for (int o = 16; o; o >>= 1) {
+      const long long h = __shfl_xor_sync(0xffffffffu, hi[c], o), l = __shfl_xor_sync(0xffffffffu, lo[c], o);
+      hi[c] = h > hi[c] ? h : hi[c];
+      lo[c] = l < lo[c] ? l : lo[c];
     }
-    __syncthreads();
+    if (lane == 0) sm[2 * c][warp] = lo[c], sm[2 * c + 1][warp] = hi[c];
+  }
+  __syncthreads();
+  if (threadIdx.x < 2 * axes) {
+    long long v = sm[threadIdx.x][0];
+    for (int w = 1; w < 32; ++w) {
+      const long long o = sm[threadIdx.x][w];
+      v = (threadIdx.x & 1) ? (o > v ? o : v) : (o < v ? o : v);
+    }
+    host_info[blockIdx.x * 2 * axes + threadIdx.x] = v;
   }
 }
 
@@ -215,11 +222,16 @@ int pom_rope_axes(const pom_rope_axes_args* a, void* stream) {
   return check_launch();
 }
 
-int pom_pos_range(const int64_t* pos, int64_t rows, int32_t axes, int64_t* info, void* stream) {
-  if (!pos || !info) return POM_ERR_NULL;
+int32_t pom_pos_range_blocks(int64_t rows) {
+  const int64_t want = ceil_div(rows, 4096);  // four rows in flight per thread
+  return static_cast<int32_t>(want < 1 ? 1 : want < POM_POS_RANGE_BLOCKS ? want : POM_POS_RANGE_BLOCKS);
+}
+
+int pom_pos_range(const int64_t* pos, int64_t rows, int32_t axes, int64_t* host_info, void* stream) {
+  if (!pos || !host_info) return POM_ERR_NULL;
   if (rows <= 0 || axes < 1 || axes > kMaxAxes) return POM_ERR_BAD_SHAPE;
-  pos_range_kernel<<<1, 1024, 0, static_cast<cudaStream_t>(stream)>>>(
-      reinterpret_cast<const long long*>(pos), rows, axes, reinterpret_cast<long long*>(info));
+  pos_range_kernel<<<static_cast<unsigned>(pom_pos_range_blocks(rows)), 1024, 0, static_cast<cudaStream_t>(stream)>>>(
+      reinterpret_cast<const long long*>(pos), rows, axes, reinterpret_cast<long long*>(host_info));
   count_launch();
   return check_launch();
 }

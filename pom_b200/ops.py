@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import ctypes as C
 import functools
+import threading
 import weakref
 from dataclasses import dataclass
 from typing import Optional, Tuple
@@ -1161,28 +1162,57 @@ def rope_axes(x: torch.Tensor, pos: torch.Tensor, tables, transpose: bool = Fals
     return y
 
 
-_pos_range_cache = {}
+class _HostRange(threading.local):
+    """This thread's page-locked memory and events for :func:`pos_range_start`; :func:`pos_range_wait` has to follow before
+    the next start."""
+
+    def __init__(self):
+        n = _abi.POS_RANGE_BLOCKS * 2 * _abi.ROPE_MAX_AXES
+        self.buf = torch.empty((n,), dtype=torch.int64, pin_memory=True)
+        self.at = self.buf.data_ptr()
+        self.vals = (C.c_int64 * n).from_address(self.at)
+        self.events = {}  # per device
 
 
-def pos_range(pos: torch.Tensor):
-    """(min, max) per column of the (..., A) int64 positions.  One small kernel and a synchronising read the first time a
-    given tensor (object and version) is seen; later calls are answered from a cache, as :func:`rope_pos_info`'s are."""
-    _require_cuda(pos)
-    cacheable = not pos.is_inference()
-    key = id(pos)
-    ent = _pos_range_cache.get(key) if cacheable else None
-    if ent is not None and ent[0]() is pos and ent[1] == pos._version:
-        return ent[2]
+_host_range = None
+_UNWRITTEN = -(1 << 63) + 1  # (a position of this value only costs the wait for the event)
+
+
+def pos_range_start(pos: torch.Tensor) -> None:
+    """Enqueues the search for the range of every column of the contiguous (..., A) int64 positions."""
+    global _host_range
+    dev = _same_device(pos)
+    if torch.cuda.is_current_stream_capturing():
+        raise RuntimeError("positions cannot be compared with their tables inside a graph capture: do it before, and pass "
+                           "validate=False")
+    if _host_range is None:
+        _host_range = _HostRange()
+    h = _host_range
+    L = _abi.lib()
     axes = pos.shape[-1]
-    flat = pos.contiguous()
-    info = torch.empty((2 * axes,), dtype=torch.int64, device=pos.device)
-    _abi.check(_abi.lib().pom_pos_range(flat.data_ptr(), flat.numel() // axes, axes, info.data_ptr(), _abi.stream_ptr()),
-               "pom_pos_range")
-    v = info.cpu().tolist()
-    out = tuple(zip(v[::2], v[1::2]))
-    if cacheable:
-        _pos_range_cache[key] = (weakref.ref(pos, lambda _r, k=key: _pos_range_cache.pop(k, None)), pos._version, out)
-    return out
+    rows = pos.numel() // axes
+    h.count = L.pom_pos_range_blocks(rows) * 2 * axes
+    h.vals[:h.count] = [_UNWRITTEN] * h.count
+    _abi.check(L.pom_pos_range(pos.data_ptr(), rows, axes, h.at, _abi.stream_of(dev)), "pom_pos_range")
+    event = h.events.get(dev)
+    if event is None:
+        event = h.events[dev] = torch.cuda.Event()
+    event.record()
+
+
+def pos_range_wait(pos: torch.Tensor):
+    """(min, max) per column, once what :func:`pos_range_start` enqueued is done (later work of the stream need not be).
+    Looks at the host's memory for some twenty microseconds, which is long enough on a stream that is not far behind; then
+    waits for the event, which lets other threads run."""
+    h = _host_range
+    v, n, step = h.vals, h.count, 2 * pos.shape[-1]
+    for _ in range(40):
+        if _UNWRITTEN not in v[:n]:
+            break
+    else:
+        h.events[pos.get_device()].synchronize()
+    got = v[:n]
+    return tuple((min(got[a::step]), max(got[a + 1::step])) for a in range(0, step, 2))
 
 
 def fill_zero(t: torch.Tensor) -> torch.Tensor:

@@ -87,6 +87,8 @@ def test_the_library_refuses_bad_arguments_before_it_launches():
     assert L.pom_layer_norm_fwd(ctypes.byref(n), None) == -4  # bf16 weights beside float32 rows
     n.wdtype = 1
     assert L.pom_layer_norm_bwd(ctypes.byref(n), None) == -8  # no dy
+    n.stats = 20
+    assert L.pom_layer_norm_fwd(ctypes.byref(n), None) == -3
     assert L.pom_linear_fwd(ctypes.byref(m), None, None) == -1
     m.M, m.N, m.K = 4, 8, 8
     assert L.pom_linear_fwd(ctypes.byref(m), None, None) == -8

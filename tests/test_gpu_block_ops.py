@@ -401,6 +401,22 @@ def test_rope_axes_positions_outside_the_tables():
     p[0, 0] = 10  # an update in place is seen
     with pytest.raises(IndexError, match="axis 0"):
         apply_rope_axes(x, p, tables)
+    # more rows than one block looks through
+    many = torch.zeros(70000, 2, dtype=torch.int64, device="cuda")
+    x = rand(1, 70000, 32, dtype=BF, seed=6)
+    assert torch.equal(apply_rope_axes(x, many, tables), x)
+    for at, axis, bad in ((69999, 0, 10), (0, 1, 12), (40000, 1, -1), (123, 0, -(1 << 62)), (5, 1, 1 << 62)):
+        p = many.clone()
+        p[at, axis] = bad
+        with pytest.raises(IndexError, match=f"axis {axis}"):
+            apply_rope_axes(x, p, tables)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        with pytest.raises(RuntimeError, match="validate=False"):
+            apply_rope_axes(x, many, tables)
+        y = apply_rope_axes(x, many, tables, validate=False)
+    g.replay()
+    assert torch.equal(y, x)
 
 
 def test_rope_axes_notices_positions_that_change_before_backward():
@@ -419,7 +435,7 @@ def test_rope_axes_notices_positions_that_change_before_backward():
 def block_pass(t):
     """The chain that a block runs, and all gradients."""
     h = layer_norm(t["x"], t["nw"], t["nb"])
-    h = apply_rope_axes(h, t["pos"], t["tables"])
+    h = apply_rope_axes(h, t["pos"], t["tables"], validate=False)
     u = linear(h, t["w1"], t["b1"], activation="gelu")
     y = linear(u, t["w2"], t["b2"], residual=t["x"])
     grads = torch.autograd.grad(y, [t[k] for k in ("x", "nw", "nb", "w1", "b1", "w2", "b2")], t["dy"])
