@@ -207,10 +207,17 @@ __global__ void __launch_bounds__(256) linear_epilogue_kernel(const FewDev a, co
     float v[VEC];
 #pragma unroll
     for (int e = 0; e < VEC; ++e) v[e] = in.get(e);
-    for (int k = 1; k < slabs; ++k) {
-      in.ld(z + k * each + r * ldz + c);
+    for (int k = 1; k < slabs; k += 3) {  // three in flight
+      Piece<float, VEC> more[3];
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) v[e] += in.get(e);
+      for (int q = 0; q < 3; ++q)
+        if (k + q < slabs) more[q].ld(z + (k + q) * each + r * ldz + c);
+#pragma unroll
+      for (int q = 0; q < 3; ++q)
+        if (k + q < slabs) {
+#pragma unroll
+          for (int e = 0; e < VEC; ++e) v[e] += more[q].get(e);
+        }
     }
     if (wide_bias) {
       if (a.bias_f32) {

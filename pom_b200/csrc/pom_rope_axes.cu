@@ -137,13 +137,16 @@ __global__ void __launch_bounds__(1024) pos_range_kernel(const long long* __rest
     if (lane == 0) sm[2 * c][warp] = lo[c], sm[2 * c + 1][warp] = hi[c];
   }
   __syncthreads();
-  if (threadIdx.x < 2 * axes) {
-    long long v = sm[threadIdx.x][0];
-    for (int w = 1; w < 32; ++w) {
-      const long long o = sm[threadIdx.x][w];
-      v = (threadIdx.x & 1) ? (o > v ? o : v) : (o < v ? o : v);
+  if (warp < 2 * axes) {  // warp w finishes value w
+    long long v = sm[warp][lane];
+    for (int o = 16; o; o >>= 1) {
+      const long long t = __shfl_xor_sync(0xffffffffu, v, o);
+      v = (warp & 1) ? (t > v ? t : v) : (t < v ? t : v);
     }
-    host_info[blockIdx.x * 2 * axes + threadIdx.x] = v;
+    if (lane == 0) {
+      host_info[blockIdx.x * 2 * axes + warp] = v;
+      __threadfence_system();  // now, not with the end of whatever follows
+    }
   }
 }
 
@@ -223,7 +226,7 @@ int pom_rope_axes(const pom_rope_axes_args* a, void* stream) {
 }
 
 int32_t pom_pos_range_blocks(int64_t rows) {
-  const int64_t want = ceil_div(rows, 4096);  // four rows in flight per thread
+  const int64_t want = ceil_div(rows, 16384);  // the host looks at every block's values, so few blocks for few rows
   return static_cast<int32_t>(want < 1 ? 1 : want < POM_POS_RANGE_BLOCKS ? want : POM_POS_RANGE_BLOCKS);
 }
 

@@ -9,6 +9,7 @@ from __future__ import annotations
 import ctypes as C
 import functools
 import threading
+import time
 import weakref
 from dataclasses import dataclass
 from typing import Optional, Tuple
@@ -1163,19 +1164,18 @@ def rope_axes(x: torch.Tensor, pos: torch.Tensor, tables, transpose: bool = Fals
 
 
 class _HostRange(threading.local):
-    """This thread's page-locked memory and events for :func:`pos_range_start`; :func:`pos_range_wait` has to follow before
-    the next start."""
+    """This thread's page-locked memory for :func:`pos_range_start`; :func:`pos_range_wait` has to follow before the next
+    start."""
 
     def __init__(self):
         n = _abi.POS_RANGE_BLOCKS * 2 * _abi.ROPE_MAX_AXES
         self.buf = torch.empty((n,), dtype=torch.int64, pin_memory=True)
         self.at = self.buf.data_ptr()
         self.vals = (C.c_int64 * n).from_address(self.at)
-        self.events = {}  # per device
 
 
 _host_range = None
-_UNWRITTEN = -(1 << 63) + 1  # (a position of this value only costs the wait for the event)
+_UNWRITTEN = -(1 << 63) + 1  # (a position of this value only costs the wait for the stream)
 
 
 def pos_range_start(pos: torch.Tensor) -> None:
@@ -1194,23 +1194,19 @@ def pos_range_start(pos: torch.Tensor) -> None:
     h.count = L.pom_pos_range_blocks(rows) * 2 * axes
     h.vals[:h.count] = [_UNWRITTEN] * h.count
     _abi.check(L.pom_pos_range(pos.data_ptr(), rows, axes, h.at, _abi.stream_of(dev)), "pom_pos_range")
-    event = h.events.get(dev)
-    if event is None:
-        event = h.events[dev] = torch.cuda.Event()
-    event.record()
 
 
 def pos_range_wait(pos: torch.Tensor):
     """(min, max) per column, once what :func:`pos_range_start` enqueued is done (later work of the stream need not be).
-    Looks at the host's memory for some twenty microseconds, which is long enough on a stream that is not far behind; then
-    waits for the event, which lets other threads run."""
+    Looks at the host's memory for 200 us, which is long enough on a stream that is not far behind, and then waits for the
+    stream, which lets other threads run and reports what went wrong."""
     h = _host_range
     v, n, step = h.vals, h.count, 2 * pos.shape[-1]
-    for _ in range(40):
-        if _UNWRITTEN not in v[:n]:
+    end = time.monotonic() + 2e-4
+    while _UNWRITTEN in v[:n]:
+        if time.monotonic() > end:
+            torch.cuda.current_stream(pos.device).synchronize()
             break
-    else:
-        h.events[pos.get_device()].synchronize()
     got = v[:n]
     return tuple((min(got[a::step]), max(got[a + 1::step])) for a in range(0, step, 2))
 
