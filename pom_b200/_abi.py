@@ -191,6 +191,7 @@ class LayerNormArgs(C.Structure):
     ]
 
 
+LINEAR_FEW_ROWS = 32  # bf16 products of up to this many rows take any N
 ACTIVATIONS = {None: 0, "gelu": 1, "gelu_tanh": 2, "silu": 3, "relu": 4}
 
 

@@ -1,11 +1,10 @@
 """Operators of a residual block around the mixer, on the CUDA kernels of this package: layer norm, the linear map with
 bias, activation and residual, and rotary positions of several axes.
 
-The reference leaves these to ``torch.nn`` (its README builds the blocks around ``PoM`` from ``nn.LayerNorm`` and
-``nn.Linear``) and has rotary positions of one and two axes (pom/pom_rope.py:152-235).  All three take bfloat16 and
-float32 tensors, any strides (rows that do not follow one another in one step are copied), run on the tensors' device
-and current stream, are differentiable once, and may be captured into CUDA graphs.  They give the same bits on every
-run.  ``pom_b200.operators`` exports them.
+The reference leaves the first two to ``torch.nn`` and has rotary positions of one and two axes
+(pom/pom_rope.py:152-235).  All three take bfloat16 and float32 tensors, any strides (rows that do not follow one another
+in one step are copied), run on the tensors' device and current stream, are differentiable once, and may be captured into
+CUDA graphs.  They give the same bits on every run.  ``pom_b200.operators`` exports them.
 
 A backward pass is captured together with its forward pass, and, as with PyTorch's own operators, while no eager graph of
 the same leaves is alive (autograd would join the capture with the stream that such a graph was made on; it raises).
@@ -27,7 +26,7 @@ _TYPES = (torch.bfloat16, torch.float32)
 
 
 def _check_tokens(x: torch.Tensor, name: str = "x") -> None:
-    # where it lives is checked with the other tensors of the call (ops._require_cuda)
+    # where it lives is checked with the other tensors of the call (ops._same_device)
     if not isinstance(x, torch.Tensor):
         raise TypeError(f"{name} must be a tensor, got {type(x).__name__}")
     if x.dtype not in _TYPES:
@@ -154,8 +153,8 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] =
     x (..., K) and ``weight`` (N, K) of one dtype, bfloat16 or float32; ``bias`` (N,) in that dtype or float32;
     ``residual`` of the output's shape and dtype; ``activation`` None, "gelu" (exact), "gelu_tanh", "silu" or "relu".
     Sums, bias, activation and residual are float32, rounded once.  With an activation and a gradient to come, its argument
-    is kept in x's dtype.  bfloat16 widths that are not multiples of 8 are padded
-    with zeros (a copy of the operands).  Under ``torch.autocast("cuda", torch.bfloat16)`` x, ``weight`` and ``residual``
+    is kept in x's dtype.  bfloat16 widths that are not multiples of 8 are padded with zeros (a copy of the operands), but for
+    N of up to 32 rows without a gradient.  Under ``torch.autocast("cuda", torch.bfloat16)`` x, ``weight`` and ``residual``
     are cast to bfloat16 on the way in."""
     _check_tokens(x)
     _check_tokens(weight, "weight")
@@ -185,13 +184,15 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] =
         if x.dtype == torch.float32 and bias.dtype != torch.float32:
             bias = bias.float()
         bias = bias.contiguous()
-    if x.dtype == torch.bfloat16 and (K % 8 or N % 8):
+    tracked = torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad)
+                                           or (residual is not None and residual.requires_grad))
+    # the kernel for few rows takes any N; bulk copies and the backward pass do not
+    if x.dtype == torch.bfloat16 and (K % 8 or (N % 8 and (tracked or x.numel() > _abi.LINEAR_FEW_ROWS * K))):
         kp, n_pad = _pad8(K), _pad8(N)
         y = linear(F.pad(x, (0, kp)), F.pad(weight, (0, kp, 0, n_pad)), None if bias is None else F.pad(bias, (0, n_pad)),
                    activation=activation, residual=None if residual is None else F.pad(residual, (0, n_pad)))
         return y[..., :N].contiguous() if n_pad else y
-    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad) or
-                                    (residual is not None and residual.requires_grad)):
+    if tracked:
         return _Linear.apply(x, weight, bias, residual, activation)
     return ops.linear_fwd(x, weight, bias, activation, residual, False)[0]
 
@@ -258,11 +259,15 @@ def apply_rope_axes(x: torch.Tensor, positions: torch.Tensor, tables: Sequence[T
     validate = validate and pos.numel() > 0
     if validate:  # the rotation follows at once (a bad position is harmless there); only the answer is waited for
         ops.pos_range_start(pos)
-    y = _RotateAxes.apply(x, pos, tabs) if x.requires_grad and torch.is_grad_enabled() else ops.rope_axes(x, pos, tabs)
-    if validate:
-        for a, ((lo, hi), (cos, _)) in enumerate(zip(ops.pos_range_wait(pos), tabs)):
-            if lo < 0 or hi >= cos.shape[0]:
-                raise IndexError(f"positions of axis {a} span [{lo}, {hi}] but its table has {cos.shape[0]} rows")
+    found = ()
+    try:
+        y = _RotateAxes.apply(x, pos, tabs) if x.requires_grad and torch.is_grad_enabled() else ops.rope_axes(x, pos, tabs)
+    finally:
+        if validate:
+            found = ops.pos_range_wait(pos)
+    for a, ((lo, hi), (cos, _)) in enumerate(zip(found, tabs)):
+        if lo < 0 or hi >= cos.shape[0]:
+            raise IndexError(f"positions of axis {a} span [{lo}, {hi}] but its table has {cos.shape[0]} rows")
     return y
 
 

@@ -4,6 +4,9 @@
 // z is kept rounded to bf16 and its slope formed again in the backward pass: an error of 2^-9 in z moves the slope by that
 // times |z| act''(z), a quarter of what rounding the slope itself would do.  What remains is the rounding of dz, which the
 // tensor cores need.
+//
+// 32768 x 1152 -> 4608 with gelu and z: 305 us (264 without an activation, the product's own time; with erff and expf per
+// element 397), so the activation's arithmetic, not the stores, is what the product waits for.
 #pragma once
 #include "epilogues.cuh"
 #include "linear_math.cuh"

@@ -47,14 +47,14 @@ __device__ __forceinline__ void st_cluster(uint32_t addr, float a, float b, floa
 // Columns 4 j .. 4 j + 3 of row `row` of a partial tile: the rows of a warp lie side by side.
 __device__ __forceinline__ uint32_t recv_offset(int row, int j) { return static_cast<uint32_t>((j * kBM + row) * 16); }
 
-template <int BN, bool A_MN, bool B_MN>
+template <int BN, bool B_MN>  // A: K-major
 __global__ void __launch_bounds__(kClusterThreads, 1)
 gemm_cluster_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                     const __grid_constant__ CUtensorMap tmY, const __grid_constant__ CUtensorMap tmZ, const ClusterDev a,
                     int* __restrict__ status) {
   using S = ClusterSmem<BN>;
   constexpr int kABytes = kBM * kBK * 2;
-  constexpr uint32_t kIdesc = make_idesc_bf16(BN, A_MN, B_MN);
+  constexpr uint32_t kIdesc = make_idesc_bf16(BN, false, B_MN);
   extern __shared__ uint8_t smem_raw[];
   uint8_t* tiles = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* recv = tiles + S::kStages * S::kStageBytes;
@@ -110,13 +110,7 @@ gemm_cluster_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
         uint8_t* sa = tiles + stage * S::kStageBytes;
         uint8_t* sb = sa + kABytes;
         mbar_expect_tx(&full_bar[stage], S::kStageBytes);
-        if constexpr (!A_MN) {
-          tma_load_3d(sa, &tmA, &full_bar[stage], kb * kBK, row0, 0);
-        } else {
-#pragma unroll
-          for (int j = 0; j < kBM / 64; ++j)
-            tma_load_3d(sa + j * (kBK * 128), &tmA, &full_bar[stage], row0 + j * 64, kb * kBK, 0);
-        }
+        tma_load_3d(sa, &tmA, &full_bar[stage], kb * kBK, row0, 0);
         if constexpr (!B_MN) {
           tma_load_3d(sb, &tmB, &full_bar[stage], kb * kBK, col0, 0);
         } else {
@@ -142,7 +136,7 @@ gemm_cluster_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
         const uint32_t sa = smem_u32(tiles + stage * S::kStageBytes), sb = sa + kABytes;
 #pragma unroll
         for (int k16 = 0; k16 < kBK / 16; ++k16) {
-          const uint64_t da = A_MN ? make_smem_desc(sa + k16 * 2048, kBK * 128, 1024) : make_smem_desc(sa + k16 * 32, 16, 1024);
+          const uint64_t da = make_smem_desc(sa + k16 * 32, 16, 1024);
           const uint64_t db = B_MN ? make_smem_desc(sb + k16 * 2048, kBK * 128, 1024) : make_smem_desc(sb + k16 * 32, 16, 1024);
           umma_bf16(tmem, da, db, kIdesc, (kb > kb0 || k16 > 0) ? 1u : 0u);
         }
@@ -290,7 +284,7 @@ inline int max_clusters(int size) {
   const int i = size == 2 ? 1 : size == 4 ? 2 : 3;
   int n = known[i].load(std::memory_order_relaxed);
   if (n) return n;
-  auto kern = gemm_cluster_kernel<128, false, false>;
+  auto kern = gemm_cluster_kernel<128, false>;
   constexpr int smem = ClusterSmem<128>::kBytes;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(static_cast<unsigned>(64 * size));
@@ -354,7 +348,7 @@ int launch_cluster(const Operands& o, int size, ClusterDev d, int* status, cudaS
   if ((rc = make_io_map(&tmY, d.y, o.N, o.M, 1, d.ldy))) return rc;
   tmZ = tmY;  // unused without z
   if (d.z && (rc = make_io_map(&tmZ, d.z, o.N, o.M, 1, o.N))) return rc;
-  auto kern = gemm_cluster_kernel<BN, false, B_MN>;
+  auto kern = gemm_cluster_kernel<BN, B_MN>;
   constexpr int smem = ClusterSmem<BN>::kBytes;
   static_assert(smem <= 232448, "more shared memory than a CTA may have");
   static std::atomic<uint64_t> attr_set{0};

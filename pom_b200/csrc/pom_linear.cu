@@ -59,6 +59,9 @@ __device__ __forceinline__ void few_finish(const FewDev& a, int row, int n, floa
 
 constexpr int kFewWarps = 8;
 
+// Bound by the trip to the weight, not by its bytes: 1152 -> 4608 (10.6 MB) takes 8.1 us at 32 rows, and 12.3 from HBM with 1
+// to 32.  The tensor cores' rate does not matter, so mma.sync, which takes its operands from registers, is enough.
+//
 // 16 * MT rows per blockIdx.y.  A block owns 8 * NT output columns and reads their weight rows once; its warps take 32-long pieces
 // of K in turn.  Lane (g, t) holds 8 adjacent k of row g of every operand, piece t: which k of the piece the matrix
 // instruction takes for which of its own k does not matter, as long as both operands agree, so the 16 bytes a lane loads
@@ -250,6 +253,7 @@ __global__ void __launch_bounds__(256) linear_epilogue_kernel(const FewDev a, co
   }
 }
 
+// One pass, bound by HBM: 32768 x 4608 bf16 with gelu 143 to 150 us (906 MB, 6.3 TB/s), where a copy would take 138.
 // dz = dy act'(z) (ACT none: dz = dy, which is not written) and the column sums of dz over the block's rows.
 // Block = 32 column lanes of VEC columns x 8 row lanes; grid = (column blocks, row chunks).
 template <class T, int VEC, int ACT>
@@ -348,7 +352,7 @@ int check_linear(const pom_linear_args* a) {
 }
 
 // bf16 1152 -> 4608: 8.1 us at 32 rows, 13.5 at 64, where the tensor cores take 11.5; 4608 -> 1152 at 64 rows: 19.7 and 12.3
-constexpr int kFewRowsBf16 = 32, kFewRowsF32 = 16;
+constexpr int kFewRowsBf16 = POM_LINEAR_FEW_ROWS, kFewRowsF32 = 16;
 
 template <int MT>
 int launch_few_bf16(const FewDev& d, cudaStream_t st) {
@@ -455,13 +459,12 @@ BwdPlan bwd_plan(const pom_linear_args* a) {
 }
 
 // d.y = act(sum of slabs + bias) + residual in bf16 (T) or fp32.
-template <class T>
-int launch_epilogue(const FewDev& d, const float* z, int64_t ldz, int slabs, int64_t M, bool wide, cudaStream_t st) {
-  const int64_t want = ceil_div(M * (d.N / (wide ? 4 : 1)), 256), cap = 16ll * sm_count();
+template <class T, int VEC>
+int launch_epilogue(const FewDev& d, const float* z, int64_t ldz, int slabs, int64_t M, cudaStream_t st) {
+  const int64_t want = ceil_div(M * (d.N / VEC), 256), cap = 16ll * sm_count();
   const dim3 grid(static_cast<unsigned>(want < cap ? want : cap));
   const long long ld = ldz, rows = M;
-  return wide ? launched(launch_pdl(linear_epilogue_kernel<T, 4>, grid, dim3(256), 0, st, d, z, ld, slabs, rows))
-              : launched(launch_pdl(linear_epilogue_kernel<T, 1>, grid, dim3(256), 0, st, d, z, ld, slabs, rows));
+  return launched(launch_pdl(linear_epilogue_kernel<T, VEC>, grid, dim3(256), 0, st, d, z, ld, slabs, rows));
 }
 
 // g, whose output is bf16 and contiguous, whole or as slabs and their sum.
@@ -472,7 +475,7 @@ int product(pom_gemm_args g, int slabs, float* slab, int* status, cudaStream_t s
   if (rc || slabs <= 1) return rc;
   FewDev d{};
   d.y = out, d.ldy = g.N, d.N = static_cast<int>(g.N);
-  return launch_epilogue<__nv_bfloat16>(d, slab, g.N, slabs, g.M, true, st);
+  return launch_epilogue<__nv_bfloat16, 4>(d, slab, g.N, slabs, g.M, st);  // the engine takes widths of multiples of 8
 }
 
 template <class T, int VEC>
@@ -540,7 +543,9 @@ int pom_linear_fwd(const pom_linear_args* a, int* status, void* stream) {
     if (!a->bias && !a->residual && !a->z && a->act == POM_ACT_NONE) return POM_OK;
     const bool wide = a->N % 4 == 0 && a->ldy % 4 == 0 && aligned16(a->y) && aligned16(a->z) &&
                       (!a->residual || (a->ldr % 4 == 0 && aligned16(a->residual)));
-    return launch_epilogue<float>(few_dev(a), static_cast<const float*>(a->y), a->ldy, 1, a->M, wide, st);
+    const float* sums = static_cast<const float*>(a->y);
+    return wide ? launch_epilogue<float, 4>(few_dev(a), sums, a->ldy, 1, a->M, st)
+                : launch_epilogue<float, 1>(few_dev(a), sums, a->ldy, 1, a->M, st);
   }
   Operands o{a->x, a->w, a->M, a->N, a->K, a->ldx, a->ldw, 1, false, false};
   if ((rc = check_operands(o))) return rc;

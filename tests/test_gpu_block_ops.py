@@ -260,6 +260,21 @@ def test_linear_only_some_gradients():
             assert torch.equal(got[k], want[k]), (which, k)
 
 
+def test_linear_few_rows_of_any_width():
+    """Untracked products of up to 32 rows take any N without a padded copy; a residual view of any alignment."""
+    for M in (1, 16, 17, 32, 33):
+        for N in (1, 7, 130, 2369):
+            x, w, b, r, _ = linear_inputs(M, 72, N, BF, F32, seed=45)
+            wide = rand(M, N + 3, dtype=BF, seed=46)
+            for res in (None, r, wide[:, 3:]):
+                with torch.no_grad():
+                    y = linear(x, w, b, activation="gelu", residual=res)
+                z = x.double() @ w.double().t() + b.double()
+                ze = 2 * 80 * E * (x.double().abs() @ w.double().abs().t() + b.double().abs())
+                want = act_reference(z, "gelu")[0] + (0 if res is None else res.double())
+                within(y, want, 1.13 * ze + 16 * E * (z.abs() + 1) + E * want.abs(), f"{M} {N}")
+
+
 def test_linear_without_rows():
     for dtype in (BF, F32):
         x = torch.empty(2, 0, 64, device="cuda", dtype=dtype, requires_grad=True)
