@@ -368,10 +368,11 @@ int launch_few_f32(const FewDev& d, cudaStream_t st) {
   return launched(launch_pdl(linear_few_f32_kernel<MR>, dim3(static_cast<unsigned>(ceil_div(d.N, 8))), dim3(32 * kFewWarps), 0, st, d));
 }
 
-// Row chunks of linear_dz_kernel, at least 32 rows each.  Sums alone: one wave of three blocks per SM (32768 x 1152: 18 us;
-// eight blocks per SM: 22).  With dz to write: eight blocks per SM (32768 x 4608: 132 us, the rate of a copy; three: 138).
+// Row chunks of linear_dz_kernel, at least 32 rows each: one wave of the blocks that an SM holds.  Sums alone, five blocks per
+// SM, 32768 x 1152 with the sum of the chunks and from HBM: 28 us (three 34, eight 32).  With dz to write, four: 32768 x 4608
+// 154 us, 8192 x 4096 43 (three 168; five 184 and 51; six 171 and 49; eight 155 and 45).
 int dz_chunk(int64_t M, int64_t N, int vec, bool sums_only) {
-  const int64_t cols = ceil_div(N, 32 * vec), blocks = (sums_only ? 3ll : 8ll) * sm_count();
+  const int64_t cols = ceil_div(N, 32 * vec), blocks = (sums_only ? 5ll : 4ll) * sm_count();
   const int64_t want = blocks / cols > 0 ? blocks / cols : 1;
   int64_t rows = ceil_div(ceil_div(M, want), 32) * 32;
   if (ceil_div(M, rows) > 65535) rows = ceil_div(ceil_div(M, 65535), 32) * 32;
