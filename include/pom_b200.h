@@ -662,7 +662,9 @@ int pom_layer_norm_fwd(const pom_layer_norm_args* a, void* stream);
 uint64_t pom_layer_norm_bwd_workspace(const pom_layer_norm_args* a);
 int pom_layer_norm_bwd(const pom_layer_norm_args* a, void* stream);
 
-#define POM_LINEAR_FEW_ROWS 32
+/* bf16 products that the kernel for few rows takes: up to 32 rows, up to 16 where K is above POM_LINEAR_SHORT_K */
+#define POM_LINEAR_SHORT_K 2048
+#define POM_LINEAR_FEW_ROWS(K) ((K) <= POM_LINEAR_SHORT_K ? 32 : 16)
 enum { POM_ACT_NONE = 0, POM_ACT_GELU = 1, POM_ACT_GELU_TANH = 2, POM_ACT_SILU = 3, POM_ACT_RELU = 4 };
 
 /* y = act(x w^T + bias) + residual with x (M, K), w (N, K), bias (N), residual and y (M, N).
@@ -671,8 +673,8 @@ enum { POM_ACT_NONE = 0, POM_ACT_GELU = 1, POM_ACT_GELU_TANH = 2, POM_ACT_SILU =
  * with an activation needs.  Backward: dz = dy act'(z) (no activation: dz = dy, z unused), dbias = column sums of dz,
  * dw = dz^T x (N, K) and dx = dz w (M, K), both contiguous; any of the three may be NULL.  dz: NULL, or where to put it
  * (contiguous).  workspace: as many bytes as the _workspace calls say (often 0 forward), 16-byte aligned.
- * bf16: K, N and every row stride multiples of 8, 16-byte aligned addresses (forward with up to POM_LINEAR_FEW_ROWS rows:
- * only K and the rows of x and w).  float32: any; fma nonzero keeps the products
+ * bf16: K, N and every row stride multiples of 8, 16-byte aligned addresses (forward with up to POM_LINEAR_FEW_ROWS(K)
+ * rows: only K and the rows of x and w).  float32: any; fma nonzero keeps the products
  * on the FMA kernel, which needs no workspace for planes of the operands. */
 typedef struct pom_linear_args {
   const void* x;

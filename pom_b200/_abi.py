@@ -191,7 +191,11 @@ class LayerNormArgs(C.Structure):
     ]
 
 
-LINEAR_FEW_ROWS = 32  # bf16 products of up to this many rows take any N
+def linear_few_rows(k: int) -> int:
+    """bf16 products of up to this many rows take any N (POM_LINEAR_FEW_ROWS)."""
+    return 32 if k <= 2048 else 16
+
+
 ACTIVATIONS = {None: 0, "gelu": 1, "gelu_tanh": 2, "silu": 3, "relu": 4}
 
 

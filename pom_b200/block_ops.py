@@ -154,7 +154,7 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] =
     ``residual`` of the output's shape and dtype; ``activation`` None, "gelu" (exact), "gelu_tanh", "silu" or "relu".
     Sums, bias, activation and residual are float32, rounded once.  With an activation and a gradient to come, its argument
     is kept in x's dtype.  bfloat16 widths that are not multiples of 8 are padded with zeros (a copy of the operands), but for
-    N of up to 32 rows without a gradient.  Under ``torch.autocast("cuda", torch.bfloat16)`` x, ``weight`` and ``residual``
+    N of up to 16 (K up to 2048: 32) rows without a gradient.  Under ``torch.autocast("cuda", torch.bfloat16)`` x, ``weight`` and ``residual``
     are cast to bfloat16 on the way in."""
     _check_tokens(x)
     _check_tokens(weight, "weight")
@@ -187,7 +187,7 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] =
     tracked = torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad)
                                            or (residual is not None and residual.requires_grad))
     # the kernel for few rows takes any N; bulk copies and the backward pass do not
-    if x.dtype == torch.bfloat16 and (K % 8 or (N % 8 and (tracked or x.numel() > _abi.LINEAR_FEW_ROWS * K))):
+    if x.dtype == torch.bfloat16 and (K % 8 or (N % 8 and (tracked or x.numel() > _abi.linear_few_rows(K) * K))):
         kp, n_pad = _pad8(K), _pad8(N)
         y = linear(F.pad(x, (0, kp)), F.pad(weight, (0, kp, 0, n_pad)), None if bias is None else F.pad(bias, (0, n_pad)),
                    activation=activation, residual=None if residual is None else F.pad(residual, (0, n_pad)))

@@ -59,8 +59,8 @@ __device__ __forceinline__ void few_finish(const FewDev& a, int row, int n, floa
 
 constexpr int kFewWarps = 8;
 
-// Bound by the trip to the weight, not by its bytes: 1152 -> 4608 (10.6 MB) takes 8.1 us at 32 rows, and 12.3 from HBM with 1
-// to 32.  The tensor cores' rate does not matter, so mma.sync, which takes its operands from registers, is enough.
+// Bound by the trip to the weight, not by its bytes: 1152 -> 4608 (10.6 MB) takes 8.2 us from HBM at one row and the
+// same at 32, 4608 -> 1152 12.9 at one.  The tensor cores' rate does not matter, so mma.sync, which takes its operands from registers, is enough.
 //
 // 16 * MT rows per blockIdx.y.  A block owns 8 * NT output columns and reads their weight rows once; its warps take 32-long pieces
 // of K in turn.  Lane (g, t) holds 8 adjacent k of row g of every operand, piece t: which k of the piece the matrix
@@ -351,8 +351,11 @@ int check_linear(const pom_linear_args* a) {
   return POM_OK;
 }
 
-// bf16 1152 -> 4608: 8.1 us at 32 rows, 13.5 at 64, where the tensor cores take 11.5; 4608 -> 1152 at 64 rows: 19.7 and 12.3
-constexpr int kFewRowsBf16 = POM_LINEAR_FEW_ROWS, kFewRowsF32 = 16;
+// bf16, this kernel and the tensor cores, weight in HBM (in the L2), us: 1152 -> 4608 at 32 rows 13.0 (6.9) and 15.7 (9.5), at 64
+// 13.5 and 11.5 in the L2; 1024 -> 1024 at 32 rows 11.2 (4.3) and 13.3 (7.9); 2048 -> 512 15.1 (5.6) and 13.5 (7.9).  Long
+// sums with two tiles of rows wait for one trip to memory after the other: 4608 -> 1152 at 32 rows 26.9 (10.2) and 16.9 (10.4), 8192 -> 2048
+// 43.6 (16.1) and 23.4 (16.2); at 16 rows 17.9 (7.2) and 16.7 (10.4), 26.1 (10.8) and 23.5 (16.1).
+constexpr int kFewRowsF32 = 16;
 
 template <int MT>
 int launch_few_bf16(const FewDev& d, cudaStream_t st) {
@@ -388,7 +391,7 @@ uint64_t slab_bytes(int slabs, int64_t M, int64_t N) {
 
 bool few_rows(const pom_linear_args* a) {
   const int per = a->dtype == POM_BF16 ? 8 : 4;
-  return a->M <= (a->dtype == POM_BF16 ? kFewRowsBf16 : kFewRowsF32) && a->K % per == 0 && a->ldx % per == 0 &&
+  return a->M <= (a->dtype == POM_BF16 ? POM_LINEAR_FEW_ROWS(a->K) : kFewRowsF32) && a->K % per == 0 && a->ldx % per == 0 &&
          a->ldw % per == 0 && aligned16(a->x) && aligned16(a->w);
 }
 

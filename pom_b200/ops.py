@@ -1064,7 +1064,7 @@ def _linear_workspace(size, a: LinearArgs, x: torch.Tensor) -> Optional[torch.Te
 def linear_fwd(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor], act: Optional[str],
                residual: Optional[torch.Tensor], want_z: bool):
     """act(z) + residual with z = x·wᵀ + bias: (y, z), z (M, N) in x's dtype or None.  x (..., K), w (N, K), both bf16
-    (K, and with more than 32 rows or z wanted N, a multiple of 8) or both float32; ``bias`` contiguous, bf16 or float32."""
+    (K, and with more than ``_abi.linear_few_rows(K)`` rows or z wanted N, a multiple of 8) or both float32; ``bias`` contiguous, bf16 or float32."""
     dev = _same_device(x, w, bias, residual)
     bf16 = x.dtype == torch.bfloat16
     x, ldx = rows_of(x, bf16)

@@ -262,17 +262,24 @@ def test_linear_only_some_gradients():
 
 def test_linear_few_rows_of_any_width():
     """Untracked products of up to 32 rows take any N without a padded copy; a residual view of any alignment."""
-    for M in (1, 16, 17, 32, 33):
+    for M, K in ((1, 72), (16, 72), (17, 72), (32, 72), (33, 72), (32, 2048), (16, 2056), (17, 2056), (32, 2049)):
         for N in (1, 7, 130, 2369):
-            x, w, b, r, _ = linear_inputs(M, 72, N, BF, F32, seed=45)
+            x, w, b, r, _ = linear_inputs(M, K, N, BF, F32, seed=45)
             wide = rand(M, N + 3, dtype=BF, seed=46)
             for res in (None, r, wide[:, 3:]):
                 with torch.no_grad():
                     y = linear(x, w, b, activation="gelu", residual=res)
                 z = x.double() @ w.double().t() + b.double()
-                ze = 2 * 80 * E * (x.double().abs() @ w.double().abs().t() + b.double().abs())
+                ze = 2 * (K + 8) * E * (x.double().abs() @ w.double().abs().t() + b.double().abs())
                 want = act_reference(z, "gelu")[0] + (0 if res is None else res.double())
                 within(y, want, 1.13 * ze + 16 * E * (z.abs() + 1) + E * want.abs(), f"{M} {N}")
+
+
+@pytest.mark.parametrize("M", [16, 17, 24, 32, 33])
+@pytest.mark.parametrize("K, N", [(2048, 200), (2056, 200), (2056, 205), (4608, 72)])
+def test_linear_few_rows_long_sums(K, N, M):
+    x, w, b, r, dy = linear_inputs(M, K, N, BF, F32, seed=47)
+    linear_check(x, w, b, r, "silu", dy)
 
 
 def test_linear_without_rows():
