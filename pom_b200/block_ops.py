@@ -257,14 +257,14 @@ def apply_rope_axes(x: torch.Tensor, positions: torch.Tensor, tables: Sequence[T
     if not pos.is_contiguous():
         pos = pos.contiguous()
     validate = validate and pos.numel() > 0
-    if validate:  # the rotation follows at once (a bad position is harmless there); only the answer is waited for
-        ops.pos_range_start(pos)
+    # the rotation follows at once (a bad position is harmless there); only the answer is waited for
+    started = ops.pos_range_start(pos) if validate else None
     found = ()
     try:
         y = _RotateAxes.apply(x, pos, tabs) if x.requires_grad and torch.is_grad_enabled() else ops.rope_axes(x, pos, tabs)
     finally:
-        if validate:
-            found = ops.pos_range_wait(pos)
+        if started is not None:
+            found = ops.pos_range_wait(started)
     for a, ((lo, hi), (cos, _)) in enumerate(zip(found, tabs)):
         if lo < 0 or hi >= cos.shape[0]:
             raise IndexError(f"positions of axis {a} span [{lo}, {hi}] but its table has {cos.shape[0]} rows")

@@ -1163,50 +1163,55 @@ def rope_axes(x: torch.Tensor, pos: torch.Tensor, tables, transpose: bool = Fals
     return y
 
 
-class _HostRange(threading.local):
-    """This thread's page-locked memory for :func:`pos_range_start`; :func:`pos_range_wait` has to follow before the next
-    start."""
+class _HostRange:
+    """Page-locked memory that one thread's :func:`pos_range_start` gives to the kernel; ``pending``: the device whose
+    kernel may still write to it, or -1."""
 
     def __init__(self):
         n = _abi.POS_RANGE_BLOCKS * 2 * _abi.ROPE_MAX_AXES
         self.buf = torch.empty((n,), dtype=torch.int64, pin_memory=True)
         self.at = self.buf.data_ptr()
         self.vals = (C.c_int64 * n).from_address(self.at)
+        self.count, self.axes, self.pending = 0, 0, -1
 
 
-_host_range = None
+_host_range = threading.local()  # one _HostRange per thread, made at the thread's first use: nothing here is shared
 _UNWRITTEN = -(1 << 63) + 1  # (a position of this value only costs the wait for the stream)
 
 
-def pos_range_start(pos: torch.Tensor) -> None:
-    """Enqueues the search for the range of every column of the contiguous (..., A) int64 positions."""
-    global _host_range
+def pos_range_start(pos: torch.Tensor) -> _HostRange:
+    """Enqueues the search for the range of every column of the contiguous (..., A) int64 positions.  What it returns
+    goes to :func:`pos_range_wait`, before this thread's next start."""
     dev = _same_device(pos)
     if torch.cuda.is_current_stream_capturing():
         raise RuntimeError("positions cannot be compared with their tables inside a graph capture: do it before, and pass "
                            "validate=False")
-    if _host_range is None:
-        _host_range = _HostRange()
-    h = _host_range
+    h = getattr(_host_range, "own", None)
+    if h is None:
+        h = _host_range.own = _HostRange()
+    elif h.pending >= 0:  # the call before was interrupted (Ctrl-C) before its wait: its kernel writes to the same memory
+        torch.cuda.synchronize(h.pending)
     L = _abi.lib()
-    axes = pos.shape[-1]
-    rows = pos.numel() // axes
-    h.count = L.pom_pos_range_blocks(rows) * 2 * axes
+    h.axes = pos.shape[-1]
+    rows = pos.numel() // h.axes
+    h.count = L.pom_pos_range_blocks(rows) * 2 * h.axes
     h.vals[:h.count] = [_UNWRITTEN] * h.count
-    _abi.check(L.pom_pos_range(pos.data_ptr(), rows, axes, h.at, _abi.stream_of(dev)), "pom_pos_range")
+    h.pending = dev
+    _abi.check(L.pom_pos_range(pos.data_ptr(), rows, h.axes, h.at, _abi.stream_of(dev)), "pom_pos_range")
+    return h
 
 
-def pos_range_wait(pos: torch.Tensor):
+def pos_range_wait(h: _HostRange):
     """(min, max) per column, once what :func:`pos_range_start` enqueued is done (later work of the stream need not be).
     Looks at the host's memory for 200 us, which is long enough on a stream that is not far behind, and then waits for the
     stream, which lets other threads run and reports what went wrong."""
-    h = _host_range
-    v, n, step = h.vals, h.count, 2 * pos.shape[-1]
+    v, n, step = h.vals, h.count, 2 * h.axes
     end = time.monotonic() + 2e-4
     while _UNWRITTEN in v[:n]:
         if time.monotonic() > end:
-            torch.cuda.current_stream(pos.device).synchronize()
+            torch.cuda.current_stream(h.pending).synchronize()
             break
+    h.pending = -1
     got = v[:n]
     return tuple((min(got[a::step]), max(got[a + 1::step])) for a in range(0, step, 2))
 
