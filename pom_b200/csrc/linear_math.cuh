@@ -74,6 +74,8 @@ __device__ __forceinline__ F2 linear_slope2(int kind, F2 z) {
     if (kind == POM_ACT_GELU)
       return fmaf(x * 0.3989422804014327f, expf(-0.5f * x * x), 0.5f * (1.f + erff(x * 0.70710678118654752f)));
     if (kind == POM_ACT_GELU_TANH) {
+      // beyond +-16 the slope is 1 or 0 to the last bit, and x^2 of far values would overflow into 0 * inf (NaN passes)
+      x = x > 16.f ? 16.f : x < -16.f ? -16.f : x;
       const float x2 = x * x, s = linear_sigmoid<FAST>(1.5957691216057308f * x * fmaf(0.044715f, x2, 1.f));
       return s * fmaf(x * (1.f - s), 1.5957691216057308f * fmaf(0.134145f, x2, 1.f), 1.f);
     }
