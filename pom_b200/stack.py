@@ -53,6 +53,8 @@ class PoMStack(nn.Module):
         """h + W2·act(W1·norm(h) + b1) + b2."""
         up, down = self.ffn_in[i], self.ffn_out[i]
         u = linear(self._normed(self.norm_ffn, i, h), up.weight, up.bias, activation=self.activation)
+        if h.dtype == torch.float32 and PoM._autocast_dtype() is not None:
+            return h + linear(u, down.weight, down.bias)  # the fused add would round the tokens with the operands
         return linear(u, down.weight, down.bias, residual=h)
 
     def _feed_forward_infer(self, i: int, h: torch.Tensor) -> torch.Tensor:
@@ -99,7 +101,8 @@ class PoMStack(nn.Module):
     @on_tensor_device
     def train_forward(self, x: torch.Tensor, mask=None) -> torch.Tensor:
         """The whole stack over (B, N, D) tokens with a backward pass, in bfloat16 or float32 (or under autocast to
-        bfloat16 over float32 parameters).  ``mask`` as in ``PoM.forward``: None, "causal", a (B, N) or (B, N, N) tensor,
+        bfloat16 over float32 parameters: products in bfloat16, while float32 tokens and their gradient stay float32 along
+        the residual path, as with ``torch.nn``).  ``mask`` as in ``PoM.forward``: None, "causal", a (B, N) or (B, N, N) tensor,
         or ``BlockCausal(frame_len)`` for the pattern of :meth:`forward`."""
         if x.dtype not in (torch.bfloat16, torch.float32) or not x.is_cuda:
             raise TypeError("PoMStack runs on CUDA bfloat16 or float32 tensors")
