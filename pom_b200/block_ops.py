@@ -3,8 +3,8 @@ bias, activation and residual, and rotary positions of several axes.
 
 The reference leaves the first two to ``torch.nn`` and has rotary positions of one and two axes
 (pom/pom_rope.py:152-235).  All three take bfloat16 and float32 tensors, any strides (rows that do not follow one another
-in one step are copied), run on the tensors' device and current stream, are differentiable once, and may be captured into
-CUDA graphs.  They give the same bits on every run.  ``pom_b200.operators`` exports them.
+in one step are copied), run on the tensors' device and current stream, are differentiable once (backward; a forward-mode tangent is refused), and may be captured
+into CUDA graphs.  They give the same bits on every run.  ``pom_b200.operators`` exports them.
 
 A backward pass is captured together with its forward pass, and, as with PyTorch's own operators, while no eager graph of
 the same leaves is alive (autograd would join the capture with the stream that such a graph was made on; it raises).
@@ -16,6 +16,7 @@ from typing import Optional, Sequence, Tuple
 
 import torch
 import torch.nn.functional as F
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _abi, ops
@@ -36,13 +37,22 @@ def _check_tokens(x: torch.Tensor, name: str = "x") -> None:
 _current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 
 
+def _has_tangent(t) -> bool:
+    if isinstance(t, torch.Tensor):
+        return forward_ad.unpack_dual(t).tangent is not None
+    return isinstance(t, (tuple, list)) and any(_has_tangent(e) for e in t)
+
+
 def _entry(fn):
-    """``eager_only`` and a switch to the device of the first argument, as the package's other entry points make it; one
-    wrapper of few steps, because a small call costs the host more than the GPU."""
+    """``eager_only``, a refusal of forward-mode derivatives (untracked calls do not go through autograd, which would refuse
+    them), and a switch to the device of the first argument, as the package's other entry points make it; one wrapper of
+    few steps, because a small call costs the host more than the GPU."""
 
     @eager_only
     @functools.wraps(fn)
     def wrapper(x, *args, **kwargs):
+        if getattr(forward_ad, "_current_level", 0) >= 0 and _has_tangent((x, *args, *kwargs.values())):
+            raise NotImplementedError(f"{fn.__name__} has no forward-mode derivative: differentiate it backward")
         if isinstance(x, torch.Tensor):
             i = x.get_device()
             if i >= 0 and i != _current_device():
