@@ -62,7 +62,7 @@ constexpr int kFewWarps = 8;
 // Bound by the trip to the weight, not by its bytes: 1152 -> 4608 (10.6 MB) takes 8.2 us from HBM at one row and the
 // same at 32, 4608 -> 1152 12.9 at one.  The tensor cores' rate does not matter, so mma.sync, which takes its operands from registers, is enough.
 //
-// 16 * MT rows per blockIdx.y.  A block owns 8 * NT output columns and reads their weight rows once; its warps take 32-long pieces
+// Up to 16 * MT rows.  A block owns 8 * NT output columns and reads their weight rows once; its warps take 32-long pieces
 // of K in turn.  Lane (g, t) holds 8 adjacent k of row g of every operand, piece t: which k of the piece the matrix
 // instruction takes for which of its own k does not matter, as long as both operands agree, so the 16 bytes a lane loads
 // are two instructions' fragments as they are.
@@ -73,7 +73,7 @@ __global__ void __launch_bounds__(32 * kFewWarps) linear_few_bf16_kernel(const F
   griddep_wait();
   griddep_launch();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const int n0 = blockIdx.x * 8 * NT, m0 = blockIdx.y * 16 * MT;
+  const int n0 = blockIdx.x * 8 * NT;
   const __nv_bfloat16* w = static_cast<const __nv_bfloat16*>(a.w);
   const __nv_bfloat16* x = static_cast<const __nv_bfloat16*>(a.x);
   float c[MT][NT][4];
@@ -99,7 +99,7 @@ __global__ void __launch_bounds__(32 * kFewWarps) linear_few_bf16_kernel(const F
       for (int i = 0; i < MT; ++i)
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          const int m = m0 + i * 16 + h * 8 + g;
+          const int m = i * 16 + h * 8 + g;
           xv[u][i][h] = ok && m < a.M ? __ldg(reinterpret_cast<const uint4*>(x + m * a.ldx + k)) : zero;
         }
     }
@@ -125,11 +125,11 @@ __global__ void __launch_bounds__(32 * kFewWarps) linear_few_bf16_kernel(const F
   __syncthreads();
   for (int i = threadIdx.x; i < 16 * MT * 8 * NT; i += 32 * kFewWarps) {
     const int m = i / (8 * NT), n = i - m * (8 * NT);
-    if (m0 + m >= a.M || n0 + n >= a.N) continue;
+    if (m >= a.M || n0 + n >= a.N) continue;
     float z = 0.f;
 #pragma unroll
     for (int q = 0; q < kFewWarps; ++q) z += red[q][m][n];
-    few_finish<__nv_bfloat16>(a, m0 + m, n0 + n, z);
+    few_finish<__nv_bfloat16>(a, m, n0 + n, z);
   }
 }
 
@@ -359,15 +359,16 @@ constexpr int kFewRowsF32 = 16;
 
 template <int MT>
 int launch_few_bf16(const FewDev& d, cudaStream_t st) {
-  const unsigned rows = static_cast<unsigned>(ceil_div(d.M, 16 * MT));
+  if (d.M > 16 * MT) return POM_ERR_TOO_LARGE;  // the kernel knows no more rows than its tiles hold
   // two column tiles per block once that still gives every SM a block: x is read half as often
   if (d.N >= 16 * sm_count())
-    return launched(launch_pdl(linear_few_bf16_kernel<MT, 2>, dim3(static_cast<unsigned>(ceil_div(d.N, 16)), rows), dim3(32 * kFewWarps), 0, st, d));
-  return launched(launch_pdl(linear_few_bf16_kernel<MT, 1>, dim3(static_cast<unsigned>(ceil_div(d.N, 8)), rows), dim3(32 * kFewWarps), 0, st, d));
+    return launched(launch_pdl(linear_few_bf16_kernel<MT, 2>, dim3(static_cast<unsigned>(ceil_div(d.N, 16))), dim3(32 * kFewWarps), 0, st, d));
+  return launched(launch_pdl(linear_few_bf16_kernel<MT, 1>, dim3(static_cast<unsigned>(ceil_div(d.N, 8))), dim3(32 * kFewWarps), 0, st, d));
 }
 
 template <int MR>
 int launch_few_f32(const FewDev& d, cudaStream_t st) {
+  if (d.M > MR) return POM_ERR_TOO_LARGE;
   return launched(launch_pdl(linear_few_f32_kernel<MR>, dim3(static_cast<unsigned>(ceil_div(d.N, 8))), dim3(32 * kFewWarps), 0, st, d));
 }
 
