@@ -671,8 +671,8 @@ enum { POM_ACT_NONE = 0, POM_ACT_GELU = 1, POM_ACT_GELU_TANH = 2, POM_ACT_SILU =
  *
  * Forward: z, where given, receives x w^T + bias as contiguous (M, N) values of dtype: what the backward call of a product
  * with an activation needs.  Backward: dz = dy act'(z) (no activation: dz = dy, z unused), dbias = column sums of dz,
- * dw = dz^T x (N, K) and dx = dz w (M, K), both contiguous; any of the three may be NULL.  dz: NULL, or where to put it
- * (contiguous).  workspace: as many bytes as the _workspace calls say (often 0 forward), 16-byte aligned.
+ * dw = dz^T x (N, K) and dx = dz w (M, K), both contiguous; any of the three may be NULL.  workspace: as many bytes as the
+ * _workspace calls say (often 0 forward), 16-byte aligned.
  * bf16: K, N and every row stride multiples of 8, 16-byte aligned addresses (forward with up to POM_LINEAR_FEW_ROWS(K)
  * rows: only K and the rows of x and w).  float32: any; fma nonzero keeps the products
  * on the FMA kernel, which needs no workspace for planes of the operands. */
@@ -684,7 +684,6 @@ typedef struct pom_linear_args {
   void* y;
   void* z;
   const void* dy;
-  void* dz;
   void* dx;
   void* dw;
   void* dbias;

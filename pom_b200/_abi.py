@@ -203,7 +203,7 @@ class LinearArgs(C.Structure):
     _fields_ = [
         ("x", C.c_void_p), ("w", C.c_void_p), ("bias", C.c_void_p), ("residual", C.c_void_p), ("y", C.c_void_p),
         ("z", C.c_void_p),
-        ("dy", C.c_void_p), ("dz", C.c_void_p), ("dx", C.c_void_p), ("dw", C.c_void_p), ("dbias", C.c_void_p),
+        ("dy", C.c_void_p), ("dx", C.c_void_p), ("dw", C.c_void_p), ("dbias", C.c_void_p),
         ("workspace", C.c_void_p),
         ("M", C.c_int64), ("N", C.c_int64), ("K", C.c_int64),
         ("ldx", C.c_int64), ("ldw", C.c_int64), ("ldr", C.c_int64), ("ldy", C.c_int64), ("ld_dy", C.c_int64),

@@ -255,7 +255,8 @@ __global__ void __launch_bounds__(256) linear_epilogue_kernel(const FewDev a, co
 
 // One pass, bound by HBM: 32768 x 4608 bf16 with gelu 143 to 150 us (906 MB, 6.3 TB/s), where a copy would take 138.
 // dz = dy act'(z) (ACT none: dz = dy, which is not written) and the column sums of dz over the block's rows.
-// Block = 32 column lanes of VEC columns x 8 row lanes; grid = (column blocks, row chunks).
+// Block = 32 column lanes of VEC columns x 8 row lanes; grid = (column blocks, row chunks).  bf16 comes in whole 16-byte pieces
+// (the products behind it want that anyway), float32 also in single values.
 template <class T, int VEC, int ACT>
 __global__ void __launch_bounds__(256) linear_dz_kernel(const T* __restrict__ dy, long long ld_dy, const T* __restrict__ z,
                                                         T* __restrict__ dz, float* __restrict__ partial, long long M, int N,
@@ -442,14 +443,14 @@ struct BwdPlan {
 BwdPlan bwd_plan(const pom_linear_args* a) {
   BwdPlan p{};
   const int per = a->dtype == POM_BF16 ? 8 : 4;
-  p.vec = a->N % per || a->ld_dy % per || !aligned16(a->dy) || !aligned16(a->z) ? 1 : per;
+  p.vec = a->N % per || a->ld_dy % per || !aligned16(a->dy) || !aligned16(a->z) ? 1 : per;  // bf16: refused unless wide
   p.chunk = dz_chunk(a->M, a->N, p.vec, a->act == POM_ACT_NONE);
   p.chunks = static_cast<int>(ceil_div(a->M, p.chunk));
   const bool bf16 = a->dtype == POM_BF16;
   p.dw_slabs = bf16 && a->dw ? gemm_bf16_slabs(a->N, a->K, a->M, true, true) : 1;
   uint64_t at = 0;
   p.dz = at;
-  if (a->act != POM_ACT_NONE && !a->dz) at = up256(at + static_cast<uint64_t>(a->M) * a->N * (bf16 ? 2 : 4));
+  if (a->act != POM_ACT_NONE) at = up256(at + static_cast<uint64_t>(a->M) * a->N * (bf16 ? 2 : 4));
   p.partial = at;
   if (a->dbias) at = up256(at + static_cast<uint64_t>(p.chunks) * a->N * 4);
   p.slab = at;
@@ -509,7 +510,7 @@ int dz_and_bias(const pom_linear_args* a, const BwdPlan& p, void* dz, cudaStream
   float* partial = a->dbias ? reinterpret_cast<float*>(static_cast<char*>(a->workspace) + p.partial) : nullptr;
   const int N = static_cast<int>(a->N);
   const int rc = a->dtype == POM_BF16
-                     ? (p.vec == 8 ? launch_dz<__nv_bfloat16, 8>(a, p, dz, partial, st) : launch_dz<__nv_bfloat16, 1>(a, p, dz, partial, st))
+                     ? launch_dz<__nv_bfloat16, 8>(a, p, dz, partial, st)
                      : (p.vec == 4 ? launch_dz<float, 4>(a, p, dz, partial, st) : launch_dz<float, 1>(a, p, dz, partial, st));
   if (rc || !partial) return rc;
   return sum_rows(partial, p.chunks, N, N, a->bias_dtype, a->dbias, nullptr, st);
@@ -591,14 +592,16 @@ int pom_linear_bwd(const pom_linear_args* a, int* status, void* stream) {
   if (a->ld_dy < a->N || (a->dx && a->ldw < a->K) || (a->dw && a->ldx < a->K)) return POM_ERR_BAD_STRIDE;
   const BwdPlan p = bwd_plan(a);
   if (p.total && !a->workspace) return POM_ERR_NULL;
-  if (!aligned16(a->workspace) || !aligned16(a->dz)) return POM_ERR_BAD_ALIGN;
-  if (a->dtype == POM_BF16 && (!aligned16(a->dw) || !aligned16(a->dx))) return POM_ERR_BAD_ALIGN;
+  if (!aligned16(a->workspace)) return POM_ERR_BAD_ALIGN;
+  if (a->dtype == POM_BF16) {
+    if (p.vec == 1 && (a->N % 8 || a->ld_dy % 8)) return POM_ERR_BAD_STRIDE;
+    if (p.vec == 1 || !aligned16(a->dw) || !aligned16(a->dx)) return POM_ERR_BAD_ALIGN;
+  }
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   char* ws = static_cast<char*>(a->workspace);
-  void* own_dz = a->dz ? a->dz : ws + p.dz;
-  if ((rc = dz_and_bias(a, p, own_dz, st))) return rc;
+  if ((rc = dz_and_bias(a, p, ws + p.dz, st))) return rc;
   const bool own = a->act != POM_ACT_NONE;
-  const void* dz = own ? own_dz : a->dy;
+  const void* dz = own ? ws + p.dz : a->dy;
   const int64_t ld_dz = own ? a->N : a->ld_dy;
   pom_gemm_args g{};
   g.batches = 1, g.split_k = 1, g.alpha = 1.f;
