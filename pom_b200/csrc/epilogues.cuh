@@ -248,6 +248,7 @@ struct EpiCtx {
     float w = 1.f;
     if (weighted)
       w = row_ok ? __ldg(p.row_weight + static_cast<long long>(t.b) * g.rows_per_batch + t.row0 + row) : 0.f;
+    if (lane == 0) bulk_wait_read<0>();  // a tile with an odd number of chunks ended on the block that this one begins with
     int flip = 0;
 #pragma unroll 1
     for (int c = half; c < BN / 32; c += kEpiColSplit) {
@@ -348,6 +349,7 @@ struct EpiGate {
                                              EpiIO& io, int iter) {
     const float* cst = scratch + (iter & 1) * 512;
     const int y = t.row0 + quarter * 32;
+    if (lane == 0) bulk_wait_read<0>();  // a tile with an odd number of chunks ended on the block that this one begins with
     int flip = 0;
 #pragma unroll 1
     for (int c = half; c < BN / 32; c += kEpiColSplit) {

@@ -311,6 +311,7 @@ struct EpiCtxRope {
     if (weighted)
       w = row < t.rows_valid ? __ldg(p.row_weight + static_cast<long long>(t.b) * g.rows_per_batch + t.row0 + row) : 0.f;
     const int y = t.row0 + quarter * 32;
+    if (lane == 0) bulk_wait_read<0>();  // a tile with an odd number of units ended on the block that this one begins with
     int flip = 0;
 #pragma unroll 1
     for (int su = half; su < BN / 32; su += kEpiColSplit) {
