@@ -234,10 +234,13 @@ def apply_rope_axes(x: torch.Tensor, positions: torch.Tensor, tables: Sequence[T
     x (B, N, D), or (B, N, H, D) with heads that share the angles.  ``tables``: per axis a (cos, sin) pair of
     (rows, s_a) tensors (see :func:`precompute_freqs_axes`); the axes' sections of 2 s_a channels follow one another, and
     inside a section channel k pairs with k + s_a, as :func:`apply_rope_2d` pairs its two halves; channels behind the
-    last section pass.  ``positions`` (N, A) for all samples, or (B, N, A).  Only x has a gradient.
+    last section pass.  ``positions`` (N, A) for all samples, or (B, N, A).  Only x has a gradient.  Tables and positions
+    of another device or type are copied in every call.
 
     ``validate``: an IndexError for a position outside its table, for which the call waits until the stream has come
-    to it (and cannot be captured).  Without it nothing is read back, and such a position makes its section of the token NaN."""
+    to it (and cannot be captured).  Without it nothing is read back, and such a position makes its section of the token
+    NaN.  Nothing is remembered between calls: a model that rotates by the same positions in every layer checks them in
+    its first call and passes ``validate=False`` in the others, so that only one call waits."""
     _check_tokens(x)
     if x.dim() not in (3, 4):
         raise ValueError(f"expected a (B, N, D) or (B, N, H, D) tensor, got {tuple(x.shape)}")
@@ -281,13 +284,13 @@ def apply_rope_axes(x: torch.Tensor, positions: torch.Tensor, tables: Sequence[T
     return y
 
 
-def precompute_freqs_axes(pairs: Sequence[int], rows: Sequence[int], base: float = 10000.0):
+def precompute_freqs_axes(pairs: Sequence[int], rows: Sequence[int], base: float = 10000.0, *, device=None):
     """One (cos, sin) pair of (rows[a], pairs[a]) float32 tables per axis, angle position * base^(-k / pairs[a]); formed in
-    64 bits, so that far positions keep their angles.  With equal axes the tables of
+    64 bits, so that far positions keep their angles.  They are wanted on the ``device`` of the tokens: made once, there.  With equal axes the tables of
     :func:`pom_b200.pom_rope.precompute_freqs_2d`."""
     out = []
     for s, n in zip(pairs, rows):
         f = float(base) ** (-torch.arange(s, dtype=torch.float64) / s)
         ang = torch.outer(torch.arange(n, dtype=torch.float64), f)
-        out.append((ang.cos().float(), ang.sin().float()))
+        out.append((ang.cos().float().to(device), ang.sin().float().to(device)))
     return out
