@@ -136,7 +136,7 @@ class _Linear(torch.autograd.Function):
     def forward(ctx, x, weight, bias, residual, act):
         nx, nw, nb, _, _ = ctx.needs_input_grad
         y, z = ops.linear_fwd(x, weight, bias, act, residual, act is not None and (nx or nw or nb))
-        ctx.save_for_backward(x, weight, z)
+        ctx.save_for_backward(x if nw else None, weight if nx else None, z)
         ctx.act = act
         ctx.bias_dtype = bias.dtype if nb else None
         return y

@@ -1034,13 +1034,6 @@ def layer_norm_bwd(dy: torch.Tensor, x: torch.Tensor, weight: Optional[torch.Ten
     return dx, dw, db
 
 
-def _linear_args(x, w, act, M, N, K, ldx, ldw) -> LinearArgs:
-    a = LinearArgs()
-    a.x, a.w, a.M, a.N, a.K, a.ldx, a.ldw = x.data_ptr(), w.data_ptr(), M, N, K, ldx, ldw
-    a.act, a.dtype = _abi.ACTIVATIONS[act], _DTYPE[x.dtype]
-    return a
-
-
 def _linear_workspace(size, a: LinearArgs, x: torch.Tensor) -> Optional[torch.Tensor]:
     """Workspace of as many bytes as ``size`` asks for.  Where memory has no room for the planes of float32 operands, the
     FMA kernel, which needs none."""
@@ -1075,7 +1068,9 @@ def linear_fwd(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor], a
     z = x.new_empty((M, N)) if want_z else None
     if M == 0:
         return y, z
-    a = _linear_args(x, w, act, M, N, K, ldx, ldw)
+    a = LinearArgs()
+    a.x, a.w, a.M, a.N, a.K, a.ldx, a.ldw = x.data_ptr(), w.data_ptr(), M, N, K, ldx, ldw
+    a.act, a.dtype = _abi.ACTIVATIONS[act], _DTYPE[x.dtype]
     a.y, a.ldy = y.data_ptr(), N
     if bias is not None:
         a.bias, a.bias_dtype = bias.data_ptr(), _DTYPE[bias.dtype]
@@ -1091,23 +1086,29 @@ def linear_fwd(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor], a
     return y, z
 
 
-def linear_bwd(dy: torch.Tensor, x: torch.Tensor, w: torch.Tensor, act: Optional[str], z: Optional[torch.Tensor], *,
-               want_dx: bool, want_dw: bool, bias_dtype: Optional[torch.dtype]):
-    """(dx, dw, dbias) of :func:`linear_fwd` (dbias where ``bias_dtype`` is given); what is not wanted is None."""
+def linear_bwd(dy: torch.Tensor, x: Optional[torch.Tensor], w: Optional[torch.Tensor], act: Optional[str],
+               z: Optional[torch.Tensor], *, want_dx: bool, want_dw: bool, bias_dtype: Optional[torch.dtype]):
+    """(dx, dw, dbias) of :func:`linear_fwd` (dbias where ``bias_dtype`` is given); what is not wanted is None.  ``x`` is
+    read only for dw and ``w`` only for dx: the other may be None."""
     dev = _same_device(dy, x, w, z)
-    bf16 = x.dtype == torch.bfloat16
-    x, ldx = rows_of(x, bf16)
-    w, ldw = rows_of(w, bf16)
-    N, K = w.shape
-    M = x.numel() // K
-    dx = (torch.empty_like(x) if ldx == K else x.new_empty(x.shape)) if want_dx else None
-    dw = w.new_empty((N, K)) if want_dw else None
-    db = w.new_empty(N, dtype=bias_dtype) if bias_dtype is not None else None
+    bf16 = dy.dtype == torch.bfloat16
+    N = dy.shape[-1]
+    M = dy.numel() // N
+    a = LinearArgs()
+    K = 1
+    if want_dw:
+        x, a.ldx = rows_of(x, bf16)
+        a.x, K = x.data_ptr(), x.shape[-1]
+    if want_dx:
+        w, a.ldw = rows_of(w, bf16)
+        a.w, K = w.data_ptr(), w.shape[-1]
+    dx = dy.new_empty((*dy.shape[:-1], K)) if want_dx else None
+    dw = dy.new_empty((N, K)) if want_dw else None
+    db = dy.new_empty(N, dtype=bias_dtype) if bias_dtype is not None else None
     if M == 0:
         return dx, dw if dw is None else fill_zero(dw), db if db is None else fill_zero(db)
-    dy, ldg = rows_of(dy, bf16)
-    a = _linear_args(x, w, act, M, N, K, ldx, ldw)
-    a.dy, a.ld_dy = dy.data_ptr(), ldg
+    dy, a.ld_dy = rows_of(dy, bf16)
+    a.M, a.N, a.K, a.act, a.dtype, a.dy = M, N, K, _abi.ACTIVATIONS[act], _DTYPE[dy.dtype], dy.data_ptr()
     if z is not None:
         a.z = z.data_ptr()
     if db is not None:
@@ -1117,7 +1118,7 @@ def linear_bwd(dy: torch.Tensor, x: torch.Tensor, w: torch.Tensor, act: Optional
     if dw is not None:
         a.dw = dw.data_ptr()
     L = _abi.lib()
-    ws = _linear_workspace(L.pom_linear_bwd_workspace, a, x)  # noqa: F841 (alive until the call below)
+    ws = _linear_workspace(L.pom_linear_bwd_workspace, a, dy)  # noqa: F841 (alive until the call below)
     _abi.check(L.pom_linear_bwd(C.byref(a), _abi.status_ptr(dev), _abi.stream_of(dev)), "pom_linear_bwd")
     return dx, dw, db
 
