@@ -1170,7 +1170,7 @@ class _HostRange:
 
     def __init__(self):
         n = _abi.POS_RANGE_BLOCKS * 2 * _abi.ROPE_MAX_AXES
-        self.buf = torch.empty((n,), dtype=torch.int64, pin_memory=True)
+        self.buf = torch.empty((n,), dtype=torch.int64, device="cpu", pin_memory=True)
         self.at = self.buf.data_ptr()
         self.vals = (C.c_int64 * n).from_address(self.at)
         self.count, self.axes, self.pending = 0, 0, -1

@@ -104,3 +104,22 @@ def test_block_on_the_device_that_is_not_current(dtype):
         layer_norm(there["x"], t["nw"])
     with pytest.raises(RuntimeError, match="same GPU"):
         linear(there["x"], t["w1"])
+
+
+def test_a_default_device_does_not_move_the_host_memory():
+    """torch.set_default_device("cuda") must not decide where the range of the positions goes."""
+    tables = [(torch.ones(10, 4, device="cuda"), torch.zeros(10, 4, device="cuda"))]
+    x, pos = rand(1, 64, 16, dtype=BF), torch.full((64, 1), 7, device="cuda")
+    got = []
+
+    def work():  # a new thread: its memory is not made yet
+        try:
+            with torch.device("cuda"):
+                got.append(apply_rope_axes(x, pos, tables))
+        except Exception as e:  # noqa: BLE001
+            got.append(repr(e))
+
+    t = threading.Thread(target=work)
+    t.start()
+    t.join()
+    assert isinstance(got[0], torch.Tensor) and torch.equal(got[0], x), got
