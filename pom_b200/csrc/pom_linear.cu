@@ -73,7 +73,9 @@ __global__ void __launch_bounds__(32 * kFewWarps) linear_few_bf16_kernel(const F
   griddep_wait();
   griddep_launch();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const int n0 = blockIdx.x * 8 * NT;
+  // m0 is 0 in every launch, but the compiler does not know: with a plain 0 it keeps fewer loads in flight, and 4608 -> 1152
+  // at one row takes 18.4 us from HBM instead of 16.4 (1152 -> 1152 at 32: 12.3 instead of 10.2)
+  const int n0 = blockIdx.x * 8 * NT, m0 = blockIdx.y * 16 * MT;
   const __nv_bfloat16* w = static_cast<const __nv_bfloat16*>(a.w);
   const __nv_bfloat16* x = static_cast<const __nv_bfloat16*>(a.x);
   float c[MT][NT][4];
@@ -99,7 +101,7 @@ __global__ void __launch_bounds__(32 * kFewWarps) linear_few_bf16_kernel(const F
       for (int i = 0; i < MT; ++i)
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          const int m = i * 16 + h * 8 + g;
+          const int m = m0 + i * 16 + h * 8 + g;
           xv[u][i][h] = ok && m < a.M ? __ldg(reinterpret_cast<const uint4*>(x + m * a.ldx + k)) : zero;
         }
     }
@@ -125,11 +127,11 @@ __global__ void __launch_bounds__(32 * kFewWarps) linear_few_bf16_kernel(const F
   __syncthreads();
   for (int i = threadIdx.x; i < 16 * MT * 8 * NT; i += 32 * kFewWarps) {
     const int m = i / (8 * NT), n = i - m * (8 * NT);
-    if (m >= a.M || n0 + n >= a.N) continue;
+    if (m0 + m >= a.M || n0 + n >= a.N) continue;
     float z = 0.f;
 #pragma unroll
     for (int q = 0; q < kFewWarps; ++q) z += red[q][m][n];
-    few_finish<__nv_bfloat16>(a, m, n0 + n, z);
+    few_finish<__nv_bfloat16>(a, m0 + m, n0 + n, z);
   }
 }
 
