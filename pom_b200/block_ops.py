@@ -98,7 +98,8 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
     """``(x - mean) / sqrt(var + eps) * weight + bias`` over the last dimension, in x's dtype.
 
     x (..., D) bfloat16 or float32; ``weight`` and ``bias`` (D,) in x's dtype or float32 (``bias`` only with ``weight``).
-    Statistics and sums are float32.  A row with an infinity or a NaN comes out NaN."""
+    Statistics and sums are float32, so a row's sum and its sum of squared deviations must stay below 3e38 (values up to
+    1e15 always do).  A row with an infinity or a NaN comes out NaN."""
     _check_tokens(x)
     if x.dim() < 1 or x.shape[-1] == 0:
         raise ValueError(f"expected a (..., D) tensor with D > 0, got {tuple(x.shape)}")
@@ -162,10 +163,16 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] =
 
     x (..., K) and ``weight`` (N, K) of one dtype, bfloat16 or float32; ``bias`` (N,) in that dtype or float32;
     ``residual`` of the output's shape and dtype; ``activation`` None, "gelu" (exact), "gelu_tanh", "silu" or "relu".
-    Sums, bias, activation and residual are float32, rounded once.  With an activation and a gradient to come, its argument
-    is kept in x's dtype.  bfloat16 widths that are not multiples of 8 are padded with zeros (a copy of the operands), but for
-    N of up to 16 (K up to 2048: 32) rows without a gradient.  Under ``torch.autocast("cuda", torch.bfloat16)`` x, ``weight`` and ``residual``
-    are cast to bfloat16 on the way in."""
+    Sums, bias, activation and residual are float32, rounded once.  Under ``torch.autocast("cuda", torch.bfloat16)`` x,
+    ``weight`` and ``residual`` are cast to bfloat16 on the way in, and y is bfloat16.
+
+    Gradients: with an activation its argument z is kept in x's dtype, and dz, what comes back through the activation, is
+    rounded to it before dW = dzᵀ x and dx = dz W.  In bfloat16 those two carry two roundings instead of one (0.0024 of
+    their norm against 0.0017); without an activation dz is the incoming gradient, and nothing is added.
+
+    bfloat16 widths that are not multiples of 8 are padded with zeros (a copy of the operands), but for N of up to 16 (K up
+    to 2048: 32) rows without a gradient.  float32 products take a workspace of three bfloat16 planes per operand; where
+    memory has no room for it, they run as chains of fused multiply-adds over the whole sum, whose error grows with K."""
     _check_tokens(x)
     _check_tokens(weight, "weight")
     if activation not in _abi.ACTIVATIONS:
