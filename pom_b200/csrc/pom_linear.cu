@@ -255,7 +255,7 @@ __global__ void __launch_bounds__(256) linear_epilogue_kernel(const FewDev a, co
   }
 }
 
-// One pass, bound by HBM: 32768 x 4608 bf16 with gelu 143 to 150 us (906 MB, 6.3 TB/s), where a copy would take 138.
+// One pass, bound by HBM: 32768 x 4608 bf16 with gelu 148 to 152 us (906 MB, 6.1 TB/s), where a copy would take 138.
 // dz = dy act'(z) (ACT none: dz = dy, which is not written) and the column sums of dz over the block's rows.
 // Block = 32 column lanes of VEC columns x 8 row lanes; grid = (column blocks, row chunks).  bf16 comes in whole 16-byte pieces
 // (the products behind it want that anyway), float32 also in single values.
