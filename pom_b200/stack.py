@@ -45,6 +45,14 @@ class PoMStack(nn.Module):
         self.norm_mix = nn.ModuleList([nn.LayerNorm(dim) for _ in range(n_layers if norm else 0)])
         self.norm_ffn = nn.ModuleList([nn.LayerNorm(dim) for _ in range(n_layers if norm else 0)])
 
+    def __setstate__(self, state):
+        """A stack that was pickled whole before it could have norms and other activations."""
+        super().__setstate__(state)
+        self.__dict__.setdefault("activation", "gelu")
+        for name in ("norm_mix", "norm_ffn"):
+            if name not in self._modules:
+                setattr(self, name, nn.ModuleList())
+
     @staticmethod
     def _normed(norms: nn.ModuleList, i: int, h: torch.Tensor) -> torch.Tensor:
         return layer_norm(h, norms[i].weight, norms[i].bias, norms[i].eps) if len(norms) else h
