@@ -19,10 +19,11 @@ using namespace pomh;
 namespace {
 
 struct FewDev {
-  const void *x, *w, *bias, *residual;
+  const void *x, *w, *bias, *residual;  // bias and residual: or null (few-row kernels: see readable)
   void *y, *z;  // z (contiguous) or null
   long long ldx, ldw, ldr, ldy;
   int M, N, K, act, bias_f32;
+  int has_bias, has_residual;
 };
 
 __device__ __forceinline__ void mma_bf16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
@@ -38,20 +39,29 @@ __device__ __forceinline__ float few_bias(const FewDev& a, int n) {
                     : __bfloat162float(__ldg(static_cast<const __nv_bfloat16*>(a.bias) + n));
 }
 
-// bias, activation, residual and stores of one output value.
+// bias, activation, residual and stores of one output value of the few-row kernels.  Every thread of the block's outputs
+// comes here: the loads stand behind no condition and read addresses that exist (row and n inside the output; an operand that is
+// not there is read at the first value of x, see readable), only the stores are left out where !in.
+//
+// With `if (a.bias)` and `if (m < M)` in front of them, the instances whose threads finish two outputs of one column
+// (MT = NT = 2) faulted at an address near 0 when there was no bias and rows were missing (20 x 1016 -> 4056): the load of the
+// bias, the same for both outputs, was made outside its conditions.
 template <class T>
-__device__ __forceinline__ void few_finish(const FewDev& a, int row, int n, float z) {
+__device__ __forceinline__ void few_finish(const FewDev& a, int row, int n, bool in, float z) {
   Piece<T, 1> p;
-  z += few_bias(a, n);
+  const int nb = a.has_bias ? n : 0;
+  const float b = a.bias_f32 ? __ldg(static_cast<const float*>(a.bias) + nb)
+                             : __bfloat162float(__ldg(static_cast<const __nv_bfloat16*>(a.bias) + nb));
+  Piece<T, 1> r;
+  r.ld(static_cast<const T*>(a.residual) + (a.has_residual ? row * a.ldr + n : 0));
+  z = a.has_bias ? z + b : z;
+  float v[1] = {linear_act<Piece<T, 1>::kBf16>(a.act, z)};
+  v[0] = a.has_residual ? v[0] + r.get(0) : v[0];
+  if (!in) return;
   if (a.z) {
     const float k[1] = {z};
     p.set(k);
     p.st(static_cast<T*>(a.z) + static_cast<long long>(row) * a.N + n);
-  }
-  float v[1] = {linear_act<Piece<T, 1>::kBf16>(a.act, z)};
-  if (a.residual) {
-    p.ld(static_cast<const T*>(a.residual) + row * a.ldr + n);
-    v[0] += p.get(0);
   }
   p.set(v);
   p.st(static_cast<T*>(a.y) + row * a.ldy + n);
@@ -59,8 +69,10 @@ __device__ __forceinline__ void few_finish(const FewDev& a, int row, int n, floa
 
 constexpr int kFewWarps = 8;
 
-// Bound by the trip to the weight, not by its bytes: 1152 -> 4608 (10.6 MB) takes 8.2 us from HBM at one row and the
-// same at 32, 4608 -> 1152 12.9 at one.  The tensor cores' rate does not matter, so mma.sync, which takes its operands from registers, is enough.
+// Bound by the trip to the weight, not by its bytes: 1152 -> 4608 (10.6 MB) takes 8 us from HBM at one row and 10 at 32,
+// 4608 -> 1152 12.3 at one.  The tensor cores' rate does not matter, so mma.sync, which takes its operands from registers, is enough.
+// The operands are read without conditions, from the last row or piece where there is none, and zeroed afterwards: the loads of
+// all pieces are in flight together (behind conditions 4608 -> 1152 took 16.4 us), and none can leave its operand.
 //
 // Up to 16 * MT rows.  A block owns 8 * NT output columns and reads their weight rows once; its warps take 32-long pieces
 // of K in turn.  Lane (g, t) holds 8 adjacent k of row g of every operand, piece t: which k of the piece the matrix
@@ -73,9 +85,7 @@ __global__ void __launch_bounds__(32 * kFewWarps) linear_few_bf16_kernel(const F
   griddep_wait();
   griddep_launch();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  // m0 is 0 in every launch, but the compiler does not know: with a plain 0 it keeps fewer loads in flight, and 4608 -> 1152
-  // at one row takes 18.4 us from HBM instead of 16.4 (1152 -> 1152 at 32: 12.3 instead of 10.2)
-  const int n0 = blockIdx.x * 8 * NT, m0 = blockIdx.y * 16 * MT;
+  const int n0 = blockIdx.x * 8 * NT;
   const __nv_bfloat16* w = static_cast<const __nv_bfloat16*>(a.w);
   const __nv_bfloat16* x = static_cast<const __nv_bfloat16*>(a.x);
   float c[MT][NT][4];
@@ -95,14 +105,16 @@ __global__ void __launch_bounds__(32 * kFewWarps) linear_few_bf16_kernel(const F
 #pragma unroll
       for (int j = 0; j < NT; ++j) {
         const int n = n0 + j * 8 + g;
-        wv[u][j] = ok && n < a.N ? __ldg(reinterpret_cast<const uint4*>(w + n * a.ldw + k)) : zero;
+        const uint4 v = __ldg(reinterpret_cast<const uint4*>(w + min(n, a.N - 1) * a.ldw + min(k, a.K - 8)));
+        wv[u][j] = ok && n < a.N ? v : zero;
       }
 #pragma unroll
       for (int i = 0; i < MT; ++i)
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          const int m = m0 + i * 16 + h * 8 + g;
-          xv[u][i][h] = ok && m < a.M ? __ldg(reinterpret_cast<const uint4*>(x + m * a.ldx + k)) : zero;
+          const int m = i * 16 + h * 8 + g;
+          const uint4 v = __ldg(reinterpret_cast<const uint4*>(x + min(m, a.M - 1) * a.ldx + min(k, a.K - 8)));
+          xv[u][i][h] = ok && m < a.M ? v : zero;
         }
     }
 #pragma unroll
@@ -127,11 +139,10 @@ __global__ void __launch_bounds__(32 * kFewWarps) linear_few_bf16_kernel(const F
   __syncthreads();
   for (int i = threadIdx.x; i < 16 * MT * 8 * NT; i += 32 * kFewWarps) {
     const int m = i / (8 * NT), n = i - m * (8 * NT);
-    if (m0 + m >= a.M || n0 + n >= a.N) continue;
     float z = 0.f;
 #pragma unroll
     for (int q = 0; q < kFewWarps; ++q) z += red[q][m][n];
-    few_finish<__nv_bfloat16>(a, m0 + m, n0 + n, z);
+    few_finish<__nv_bfloat16>(a, min(m, a.M - 1), min(n0 + n, a.N - 1), m < a.M && n0 + n < a.N, z);
   }
 }
 
@@ -184,11 +195,10 @@ __global__ void __launch_bounds__(32 * kFewWarps) linear_few_f32_kernel(const Fe
   __syncthreads();
   for (int i = threadIdx.x; i < MR * 8; i += 32 * kFewWarps) {
     const int m = i >> 3, n = i & 7;
-    if (m >= a.M || n0 + n >= a.N) continue;
     float z = 0.f;
 #pragma unroll
     for (int q = 0; q < kFewWarps; ++q) z += red[q][m][n];
-    few_finish<float>(a, m, n0 + n, z);
+    few_finish<float>(a, min(m, a.M - 1), min(n0 + n, a.N - 1), m < a.M && n0 + n < a.N, z);
   }
 }
 
@@ -341,6 +351,14 @@ FewDev few_dev(const pom_linear_args* a) {
   d.ldx = a->ldx, d.ldw = a->ldw, d.ldr = a->ldr, d.ldy = a->ldy;
   d.M = static_cast<int>(a->M < INT32_MAX ? a->M : INT32_MAX), d.N = static_cast<int>(a->N), d.K = static_cast<int>(a->K);
   d.act = a->act, d.bias_f32 = a->bias_dtype == POM_F32;
+  d.has_bias = a->bias != nullptr, d.has_residual = a->residual != nullptr;
+  return d;
+}
+
+// For the few-row kernels: an operand that is not there points at x, whose first value has the tokens' type.
+FewDev readable(FewDev d, int dtype) {
+  if (!d.bias) d.bias = d.x, d.bias_f32 = dtype == POM_F32;
+  if (!d.residual) d.residual = d.x;
   return d;
 }
 
@@ -354,10 +372,10 @@ int check_linear(const pom_linear_args* a) {
   return POM_OK;
 }
 
-// bf16, this kernel and the tensor cores, weight in HBM (in the L2), us: 1152 -> 4608 at 32 rows 13.0 (6.9) and 15.7 (9.5), at 64
-// 13.5 and 11.5 in the L2; 1024 -> 1024 at 32 rows 11.2 (4.3) and 13.3 (7.9); 2048 -> 512 15.1 (5.6) and 13.5 (7.9).  Long
-// sums with two tiles of rows wait for one trip to memory after the other: 4608 -> 1152 at 32 rows 26.9 (10.2) and 16.9 (10.4), 8192 -> 2048
-// 43.6 (16.1) and 23.4 (16.2); at 16 rows 17.9 (7.2) and 16.7 (10.4), 26.1 (10.8) and 23.5 (16.1).
+// bf16, this kernel and the tensor cores, weight in HBM (in the L2), us: 1152 -> 4608 at 32 rows 10.2 (6.0) and 14.3 (8.6);
+// 1024 -> 1024 at 32 rows 8.2 (3.7) and 12.3 (7.6); 2048 -> 512 12.3 (5.2) and 12.3 (7.8).  Long sums with two tiles of rows wait
+// for one trip to memory after the other: 4608 -> 1152 at 32 rows 24.6 (11.4) and 14.3 (10.1), 8192 -> 2048 41.0 (20.6) and 20.5
+// (15.5); at 16 rows 12.3 (6.0) and 14.3 (10.1), 20.5 (9.7) and 20.5 (15.5).
 constexpr int kFewRowsF32 = 16;
 
 template <int MT>
@@ -529,7 +547,7 @@ int pom_linear_fwd(const pom_linear_args* a, int* status, void* stream) {
   if (a->ldx < a->K || a->ldw < a->K || a->ldy < a->N || (a->residual && a->ldr < a->N)) return POM_ERR_BAD_STRIDE;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (few_rows(a)) {
-    const FewDev d = few_dev(a);
+    const FewDev d = readable(few_dev(a), a->dtype);
     if (a->dtype == POM_BF16) {
       return a->M <= 16 ? launch_few_bf16<1>(d, st) : launch_few_bf16<2>(d, st);
     }
