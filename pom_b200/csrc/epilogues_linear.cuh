@@ -37,8 +37,8 @@ __device__ __forceinline__ void linear_act_row(int act, float (&v)[LEN]) {
 template <bool RES>
 struct EpiLinear {
   struct Params {
-    const void* bias;  // (N) bf16 or fp32, or null
-    int bias_f32;
+    const void* bias;  // (N) bf16 or fp32; has_bias 0: an address that may be read
+    int has_bias, bias_f32;
     int act;
     int save_z;  // maps.out0 = z; maps.out1 = y; maps.in0 = residual
   };
@@ -70,7 +70,7 @@ struct EpiLinear {
     for (int j = epi_tid; j < BN; j += kEpiThreads) {
       const int col = t.col0 + j;
       float v = 0.f;
-      if (p.bias && col < g.n_cols)
+      if (p.has_bias && col < g.n_cols)
         v = p.bias_f32 ? __ldg(static_cast<const float*>(p.bias) + col)
                        : __bfloat162float(__ldg(static_cast<const __nv_bfloat16*>(p.bias) + col));
       cst[j] = v;

@@ -18,8 +18,9 @@
 namespace pomk {
 
 struct ClusterDev {
-  const void* bias;  // (N) bf16 or fp32, or null
+  const void* bias;  // (N) bf16 or fp32
   const __nv_bfloat16* residual;
+  int has_bias, has_residual;  // 0: set to the first operand by cluster_product, an address that may be read
   __nv_bfloat16* y;
   __nv_bfloat16* z;  // contiguous, or null
   long long ldr, ldy;
@@ -156,7 +157,7 @@ gemm_cluster_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
   const int width = slice < 32 ? slice : 32;                 // columns of a chunk; a warp takes chunks half, half + 2, ...
   // residual of the eight columns at `at` of this CTA's slice (N is a multiple of 8)
   auto residual = [&](int at) {
-    if (a.residual && r < a.M && at < slice && first + at < a.N)
+    if (a.has_residual && r < a.M && at < slice && first + at < a.N)
       return __ldg(reinterpret_cast<const uint4*>(a.residual + r * a.ldr + first + at));
     return make_uint4(0, 0, 0, 0);
   };
@@ -165,7 +166,7 @@ gemm_cluster_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
     const int e = threadIdx.x - 64;
     if (e < slice) {
       float b = 0.f;
-      if (a.bias && first + e < a.N)
+      if (a.has_bias && first + e < a.N)
         b = a.bias_f32 ? __ldg(static_cast<const float*>(a.bias) + first + e)
                        : __bfloat162float(__ldg(static_cast<const __nv_bfloat16*>(a.bias) + first + e));
       bias_sm[e] = b;
@@ -377,9 +378,11 @@ int launch_cluster(const Operands& o, int size, ClusterDev d, int* status, cudaS
 }
 
 // The product with the epilogue that `d` describes (its sizes are filled in here); K-major A, either B.
-inline int cluster_product(const Operands& o, const ClusterPlan& p, const ClusterDev& d, int* status, cudaStream_t st) {
+inline int cluster_product(const Operands& o, const ClusterPlan& p, ClusterDev d, int* status, cudaStream_t st) {
   const int rc = check_operands(o);
   if (rc) return rc;
+  if (!d.has_bias) d.bias = o.A, d.bias_f32 = 0;
+  if (!d.has_residual) d.residual = static_cast<const __nv_bfloat16*>(o.A), d.ldr = 0;
   if (o.b_mn)
     return p.bn == 128 ? launch_cluster<128, true>(o, p.size, d, status, st) : launch_cluster<256, true>(o, p.size, d, status, st);
   return p.bn == 128 ? launch_cluster<128, false>(o, p.size, d, status, st) : launch_cluster<256, false>(o, p.size, d, status, st);

@@ -19,7 +19,7 @@ using namespace pomh;
 namespace {
 
 struct FewDev {
-  const void *x, *w, *bias, *residual;  // bias and residual: or null (few-row kernels: see readable)
+  const void *x, *w, *bias, *residual;  // an absent bias or residual: an address that may be read (see readable)
   void *y, *z;  // z (contiguous) or null
   long long ldx, ldw, ldr, ldy;
   int M, N, K, act, bias_f32;
@@ -34,7 +34,6 @@ __device__ __forceinline__ void mma_bf16(float (&c)[4], uint32_t a0, uint32_t a1
 }
 
 __device__ __forceinline__ float few_bias(const FewDev& a, int n) {
-  if (!a.bias) return 0.f;
   return a.bias_f32 ? __ldg(static_cast<const float*>(a.bias) + n)
                     : __bfloat162float(__ldg(static_cast<const __nv_bfloat16*>(a.bias) + n));
 }
@@ -49,9 +48,7 @@ __device__ __forceinline__ float few_bias(const FewDev& a, int n) {
 template <class T>
 __device__ __forceinline__ void few_finish(const FewDev& a, int row, int n, bool in, float z) {
   Piece<T, 1> p;
-  const int nb = a.has_bias ? n : 0;
-  const float b = a.bias_f32 ? __ldg(static_cast<const float*>(a.bias) + nb)
-                             : __bfloat162float(__ldg(static_cast<const __nv_bfloat16*>(a.bias) + nb));
+  const float b = few_bias(a, a.has_bias ? n : 0);
   Piece<T, 1> r;
   r.ld(static_cast<const T*>(a.residual) + (a.has_residual ? row * a.ldr + n : 0));
   z = a.has_bias ? z + b : z;
@@ -211,7 +208,7 @@ __global__ void __launch_bounds__(256) linear_epilogue_kernel(const FewDev a, co
   griddep_launch();
   const int per_row = a.N / VEC;
   const long long total = M * per_row, each = M * ldz;
-  const bool wide_bias = a.bias && !(reinterpret_cast<uintptr_t>(a.bias) & 15);
+  const bool wide_bias = a.has_bias && !(reinterpret_cast<uintptr_t>(a.bias) & 15);
   for (long long i = blockIdx.x * 256ll + threadIdx.x; i < total; i += gridDim.x * 256ll) {
     const long long r = total <= 0x7fffffff ? static_cast<unsigned>(i) / static_cast<unsigned>(per_row) : i / per_row;
     const int c = static_cast<int>(i - r * per_row) * VEC;
@@ -245,7 +242,7 @@ __global__ void __launch_bounds__(256) linear_epilogue_kernel(const FewDev a, co
 #pragma unroll
         for (int e = 0; e < VEC; ++e) v[e] += b.get(e);
       }
-    } else if (a.bias) {
+    } else if (a.has_bias) {
 #pragma unroll
       for (int e = 0; e < VEC; ++e) v[e] += few_bias(a, c + e);
     }
@@ -255,7 +252,7 @@ __global__ void __launch_bounds__(256) linear_epilogue_kernel(const FewDev a, co
     }
 #pragma unroll
     for (int e = 0; e < VEC; ++e) v[e] = linear_act<Piece<T, 1>::kBf16>(a.act, v[e]);
-    if (a.residual) {
+    if (a.has_residual) {
       q.ld(static_cast<const T*>(a.residual) + r * a.ldr + c);
 #pragma unroll
       for (int e = 0; e < VEC; ++e) v[e] += q.get(e);
@@ -355,10 +352,11 @@ FewDev few_dev(const pom_linear_args* a) {
   return d;
 }
 
-// For the few-row kernels: an operand that is not there points at x, whose first value has the tokens' type.
-FewDev readable(FewDev d, int dtype) {
-  if (!d.bias) d.bias = d.x, d.bias_f32 = dtype == POM_F32;
-  if (!d.residual) d.residual = d.x;
+// An absent bias or residual points at `there`, whose first value has the type `dtype`: a load that the compiler makes ahead of
+// its condition finds memory.
+FewDev readable(FewDev d, const void* there, int dtype) {
+  if (!d.has_bias) d.bias = there, d.bias_f32 = dtype == POM_F32;
+  if (!d.has_residual) d.residual = there, d.ldr = 0;
   return d;
 }
 
@@ -486,7 +484,8 @@ BwdPlan bwd_plan(const pom_linear_args* a) {
 
 // d.y = act(sum of slabs + bias) + residual in bf16 (T) or fp32.
 template <class T, int VEC>
-int launch_epilogue(const FewDev& d, const float* z, int64_t ldz, int slabs, int64_t M, cudaStream_t st) {
+int launch_epilogue(const FewDev& few, const float* z, int64_t ldz, int slabs, int64_t M, cudaStream_t st) {
+  const FewDev d = readable(few, z, POM_F32);
   const int64_t want = ceil_div(M * (d.N / VEC), 256), cap = 16ll * sm_count();
   const dim3 grid(static_cast<unsigned>(want < cap ? want : cap));
   const long long ld = ldz, rows = M;
@@ -547,7 +546,7 @@ int pom_linear_fwd(const pom_linear_args* a, int* status, void* stream) {
   if (a->ldx < a->K || a->ldw < a->K || a->ldy < a->N || (a->residual && a->ldr < a->N)) return POM_ERR_BAD_STRIDE;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (few_rows(a)) {
-    const FewDev d = readable(few_dev(a), a->dtype);
+    const FewDev d = readable(few_dev(a), a->x, a->dtype);
     if (a->dtype == POM_BF16) {
       return a->M <= 16 ? launch_few_bf16<1>(d, st) : launch_few_bf16<2>(d, st);
     }
@@ -580,8 +579,8 @@ int pom_linear_fwd(const pom_linear_args* a, int* status, void* stream) {
     if (a->N % 8 || a->ldy % 8 || (a->residual && a->ldr % 8)) return POM_ERR_BAD_STRIDE;
     if (!aligned16(a->y) || !aligned16(a->z) || !aligned16(a->residual)) return POM_ERR_BAD_ALIGN;
     ClusterDev d{};
-    d.bias = a->bias, d.bias_f32 = a->bias_dtype == POM_F32, d.act = a->act;
-    d.residual = static_cast<const __nv_bfloat16*>(a->residual), d.ldr = a->ldr;
+    d.bias = a->bias, d.has_bias = a->bias != nullptr, d.bias_f32 = a->bias_dtype == POM_F32, d.act = a->act;
+    d.residual = static_cast<const __nv_bfloat16*>(a->residual), d.has_residual = a->residual != nullptr, d.ldr = a->ldr;
     d.y = static_cast<__nv_bfloat16*>(a->y), d.ldy = a->ldy;
     d.z = static_cast<__nv_bfloat16*>(a->z);
     return cluster_product(o, cp, d, status, st);
@@ -591,10 +590,10 @@ int pom_linear_fwd(const pom_linear_args* a, int* status, void* stream) {
   if ((rc = make_io_map(&maps.out1, a->y, a->N, a->M, 1, a->ldy))) return rc;
   if (a->residual) {
     if ((rc = make_io_map(&maps.in0, a->residual, a->N, a->M, 1, a->ldr))) return rc;
-    const EpiLinear<true>::Params ep{a->bias, a->bias_dtype == POM_F32, a->act, a->z != nullptr};
+    const EpiLinear<true>::Params ep{a->bias ? a->bias : a->x, a->bias != nullptr, a->bias_dtype == POM_F32, a->act, a->z != nullptr};
     return run_plan<false, false, EpiLinear<true>>(pick_plan(o, true), o, 1, maps, ep, status, st);
   }
-  const EpiLinear<false>::Params ep{a->bias, a->bias_dtype == POM_F32, a->act, a->z != nullptr};
+  const EpiLinear<false>::Params ep{a->bias ? a->bias : a->x, a->bias != nullptr, a->bias_dtype == POM_F32, a->act, a->z != nullptr};
   return run_plan<false, false, EpiLinear<false>>(pick_plan(o, true), o, 1, maps, ep, status, st);
 }
 

@@ -19,8 +19,8 @@ namespace {
 
 struct NormDev {
   const void* x;
-  const void* w;  // or null: 1
-  const void* b;  // or null: 0
+  const void* w;  // without a scale (has_w 0): x, so that nothing is ever read at an address that does not exist
+  const void* b;  // without a shift (has_b 0): w
   void* y;
   float2* stats;  // (mean, r) per row, or null (forward)
   const void* dy;
@@ -28,6 +28,7 @@ struct NormDev {
   float* partial;  // (blocks, 2, D) or null
   long long M, ldx, ldy, ld_dy, ld_dx;
   int D;
+  int has_w, has_b;
   float eps;
 };
 
@@ -105,7 +106,7 @@ __global__ void norm_fwd_kernel(const NormDev a) {
         float o[VEC];
 #pragma unroll
         for (int e = 0; e < VEC; ++e) o[e] = (p[i].get(e) - mean) * r;
-        if (a.w) {
+        if (a.has_w) {
           constexpr int WV = VEC * static_cast<int>(sizeof(W)) <= 16 ? VEC : 16 / static_cast<int>(sizeof(W));
           const W* w = static_cast<const W*>(a.w) + c;
           const W* b = static_cast<const W*>(a.b) + c;
@@ -113,7 +114,7 @@ __global__ void norm_fwd_kernel(const NormDev a) {
           for (int k = 0; k < VEC; k += WV) {
             Piece<W, WV> pw, pb;
             pw.ld(w + k);
-            if (a.b) pb.ld(b + k);
+            if (a.has_b) pb.ld(b + k);
             else pb.zero();
 #pragma unroll
             for (int e = 0; e < WV; ++e) o[k + e] = fmaf(o[k + e], pw.get(e), pb.get(e));
@@ -150,10 +151,10 @@ __global__ void __launch_bounds__(512) norm_fwd_wide_kernel(const NormDev a) {
     for (int c = threadIdx.x; c < a.D; c += 512) {
       p.ld(x + c);
       float o[1] = {(p.get(0) - mean) * r};
-      if (a.w) {
+      if (a.has_w) {
         Piece<W, 1> pw, pb;
         pw.ld(static_cast<const W*>(a.w) + c);
-        if (a.b) pb.ld(static_cast<const W*>(a.b) + c);
+        if (a.has_b) pb.ld(static_cast<const W*>(a.b) + c);
         else pb.zero();
         o[0] = fmaf(o[0], pw.get(0), pb.get(0));
       }
@@ -195,7 +196,7 @@ __global__ void __launch_bounds__(TPR == 32 ? 384 : TPR, TPR == 128 ? 3 : 1) nor
   griddep_wait();
   griddep_launch();
   const float inv_d = 1.f / static_cast<float>(a.D);
-  const bool affine = a.w != nullptr;
+  const bool affine = a.has_w;
   for (int c = threadIdx.x; c < NV * TPR * VEC; c += T0) {
     Piece<W, 1> p;
     p.zero();
@@ -340,8 +341,8 @@ __global__ void __launch_bounds__(TPR == 32 ? 384 : TPR) norm_bwd_odd_kernel(con
   for (int i = 0; i < NV; ++i) {
     const int c = i * TPR + t;
     Piece<W, 1> p;
-    if (a.w && c < a.D) p.ld(static_cast<const W*>(a.w) + c);
-    w[i] = a.w && c < a.D ? p.get(0) : 1.f;
+    if (a.has_w && c < a.D) p.ld(static_cast<const W*>(a.w) + c);
+    w[i] = a.has_w && c < a.D ? p.get(0) : 1.f;
     dw[i] = db[i] = 0.f;
   }
   int slot = 0;
@@ -425,8 +426,8 @@ __global__ void __launch_bounds__(512) norm_bwd_wide_kernel(const NormDev a) {
     float s1 = 0.f, s2 = 0.f;
     for (int c = threadIdx.x; c < a.D; c += 512) {
       px.ld(x + c), pg.ld(g + c);
-      if (a.w) pw.ld(static_cast<const W*>(a.w) + c);
-      const float h = a.w ? pg.get(0) * pw.get(0) : pg.get(0);
+      if (a.has_w) pw.ld(static_cast<const W*>(a.w) + c);
+      const float h = a.has_w ? pg.get(0) * pw.get(0) : pg.get(0);
       s1 += h;
       s2 = fmaf(h, (px.get(0) - st.x) * st.y, s2);
     }
@@ -434,8 +435,8 @@ __global__ void __launch_bounds__(512) norm_bwd_wide_kernel(const NormDev a) {
     slot ^= 1;
     for (int c = threadIdx.x; c < a.D; c += 512) {
       px.ld(x + c), pg.ld(g + c);
-      if (a.w) pw.ld(static_cast<const W*>(a.w) + c);
-      const float h = a.w ? pg.get(0) * pw.get(0) : pg.get(0);
+      if (a.has_w) pw.ld(static_cast<const W*>(a.w) + c);
+      const float h = a.has_w ? pg.get(0) * pw.get(0) : pg.get(0);
       const float o[1] = {st.y * (h - s.x * inv_d - (px.get(0) - st.x) * st.y * (s.y * inv_d))};
       px.set(o);
       px.st(dx + c);
@@ -561,6 +562,7 @@ int norm_wide(const NormDev& d, bool bwd, cudaStream_t st) {
 }
 
 int run_norm(const NormDev& d, const NormPlan& p, int dtype, int wdtype, bool bwd, int blocks, cudaStream_t st) {
+  if (!d.has_w) wdtype = dtype;
   using B = __nv_bfloat16;
   if (dtype == POM_BF16 && wdtype == POM_BF16)
     return !p.tpr ? norm_wide<B, B>(d, bwd, st) : p.vec == 8 ? norm_any<B, B, 8>(d, p, bwd, blocks, st) : norm_any<B, B, 1>(d, p, bwd, blocks, st);
@@ -602,7 +604,9 @@ int partial_rows(const pom_layer_norm_args* a, const NormPlan& p) {
 
 NormDev norm_dev(const pom_layer_norm_args* a) {
   NormDev d;
-  d.x = a->x, d.w = a->weight, d.b = a->bias, d.y = a->y;
+  d.x = a->x, d.y = a->y;
+  d.has_w = a->weight != nullptr, d.has_b = a->bias != nullptr;
+  d.w = a->weight ? a->weight : a->x, d.b = a->bias ? a->bias : d.w;
   d.stats = reinterpret_cast<float2*>(a->stats);
   d.dy = a->dy, d.dx = a->dx, d.partial = nullptr;
   d.M = a->M, d.ldx = a->ldx, d.ldy = a->ldy, d.ld_dy = a->ld_dy, d.ld_dx = a->ld_dx;
