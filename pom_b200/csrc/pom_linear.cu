@@ -43,7 +43,7 @@ __device__ __forceinline__ float few_bias(const FewDev& a, int n) {
 // not there is read at the first value of x, see readable), only the stores are left out where !in.
 //
 // With `if (a.bias)` and `if (m < M)` in front of them, the instances whose threads finish two outputs of one column
-// (MT = NT = 2) faulted at an address near 0 when there was no bias and rows were missing (20 x 1016 -> 4056): the load of the
+// (MT = NT = 2) faulted at an unmapped address when there was no bias and rows were missing (20 x 1016 -> 4056): the load of the
 // bias, the same for both outputs, was made outside its conditions.
 template <class T>
 __device__ __forceinline__ void few_finish(const FewDev& a, int row, int n, bool in, float z) {
