@@ -123,3 +123,17 @@ def test_a_default_device_does_not_move_the_host_memory():
     t.start()
     t.join()
     assert isinstance(got[0], torch.Tensor) and torch.equal(got[0], x), got
+
+
+def test_positions_are_waited_for_on_a_stream_that_is_behind():
+    """Longer than the call looks at the host's memory: it waits for its own stream, and another stream's work does not count."""
+    tables = [(torch.ones(10, 4, device="cuda"), torch.zeros(10, 4, device="cuda"))]
+    x, good, bad = rand(1, 64, 16, dtype=BF), torch.full((64, 1), 9, device="cuda"), torch.full((64, 1), 12, device="cuda")
+    torch.cuda.synchronize()
+    for stream in (torch.cuda.current_stream(), torch.cuda.Stream()):
+        with torch.cuda.stream(stream):
+            torch.cuda._sleep(4_000_000)  # some 2 ms
+            assert torch.equal(apply_rope_axes(x, good, tables), x)
+            torch.cuda._sleep(4_000_000)
+            with pytest.raises(IndexError, match=r"\[12, 12\]"):
+                apply_rope_axes(x, bad, tables)
