@@ -3,8 +3,9 @@ bias, activation and residual, and rotary positions of several axes.
 
 The reference leaves the first two to ``torch.nn`` and has rotary positions of one and two axes
 (pom/pom_rope.py:152-235).  All three take bfloat16 and float32 tensors, any strides (rows that do not follow one another
-in one step are copied), run on the tensors' device and current stream, are differentiable once (backward; a forward-mode tangent is refused), and may be captured
-into CUDA graphs.  They give the same bits on every run.  ``pom_b200.operators`` exports them.
+in one step are copied), run on the tensors' device and current stream, are differentiable once (backward; a forward-mode
+tangent is refused), and may be captured into CUDA graphs.  They give the same bits on every run.  ``pom_b200.operators``
+exports them.
 
 A backward pass is captured together with its forward pass, and, as with PyTorch's own operators, while no eager graph of
 the same leaves is alive (autograd would join the capture with the stream that such a graph was made on; it raises).
@@ -156,6 +157,10 @@ def _pad8(n: int) -> int:
     return -n % 8
 
 
+def _padded(t: Optional[torch.Tensor], *pad: int) -> Optional[torch.Tensor]:
+    return t if t is None or not any(pad) else F.pad(t, pad)  # (padding by nothing would copy)
+
+
 @_entry
 def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None, *,
            activation: Optional[str] = None, residual: Optional[torch.Tensor] = None) -> torch.Tensor:
@@ -170,8 +175,8 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] =
     rounded to it before dW = dzᵀ x and dx = dz W.  In bfloat16 those two carry two roundings instead of one (0.0024 of
     their norm against 0.0017); without an activation dz is the incoming gradient, and nothing is added.
 
-    bfloat16 widths that are not multiples of 8 are padded with zeros (a copy of the operands), but for N of up to 16 (K up
-    to 2048: 32) rows without a gradient.  float32 products take a workspace of three bfloat16 planes per operand; where
+    bfloat16 widths that are not multiples of 8 are padded with zeros (a copy of the operands that have them), but for N
+    of up to 16 (K up to 2048: 32) rows without a gradient.  float32 products take a workspace of three bfloat16 planes per operand; where
     memory has no room for it, they run as chains of fused multiply-adds over the whole sum, whose error grows with K."""
     _check_tokens(x)
     _check_tokens(weight, "weight")
@@ -206,8 +211,8 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] =
     # the kernel for few rows takes any N; bulk copies and the backward pass do not
     if x.dtype == torch.bfloat16 and (K % 8 or (N % 8 and (tracked or x.numel() > _abi.linear_few_rows(K) * K))):
         kp, n_pad = _pad8(K), _pad8(N)
-        y = linear(F.pad(x, (0, kp)), F.pad(weight, (0, kp, 0, n_pad)), None if bias is None else F.pad(bias, (0, n_pad)),
-                   activation=activation, residual=None if residual is None else F.pad(residual, (0, n_pad)))
+        y = linear(_padded(x, 0, kp), _padded(weight, 0, kp, 0, n_pad), _padded(bias, 0, n_pad), activation=activation,
+                   residual=_padded(residual, 0, n_pad))
         return y[..., :N].contiguous() if n_pad else y
     if tracked:
         return _Linear.apply(x, weight, bias, residual, activation)
@@ -293,8 +298,8 @@ def apply_rope_axes(x: torch.Tensor, positions: torch.Tensor, tables: Sequence[T
 
 def precompute_freqs_axes(pairs: Sequence[int], rows: Sequence[int], base: float = 10000.0, *, device=None):
     """One (cos, sin) pair of (rows[a], pairs[a]) float32 tables per axis, angle position * base^(-k / pairs[a]); formed in
-    64 bits, so that far positions keep their angles.  They are wanted on the ``device`` of the tokens: made once, there.  With equal axes the tables of
-    :func:`pom_b200.pom_rope.precompute_freqs_2d`."""
+    64 bits, so that far positions keep their angles.  They are wanted on the ``device`` of the tokens: made once, there.
+    With equal axes the tables of :func:`pom_b200.pom_rope.precompute_freqs_2d`."""
     out = []
     for s, n in zip(pairs, rows):
         f = float(base) ** (-torch.arange(s, dtype=torch.float64) / s)

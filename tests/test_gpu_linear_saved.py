@@ -49,3 +49,21 @@ def test_tokens_under_a_frozen_weight_are_let_go():
     before = torch.cuda.memory_allocated()
     y = linear(x * 1, w)  # the product's input is an intermediate of 32 MB
     assert torch.cuda.memory_allocated() - before == y.numel() * 2
+
+
+def test_padding_copies_only_what_has_the_odd_width():
+    """An odd number of outputs pads the weight and the result, not the 32 MB of tokens; an odd sum pads no residual."""
+    x = torch.randn(16384, 1024, device="cuda", dtype=torch.bfloat16)
+    w = torch.randn(1001, 1024, device="cuda", dtype=torch.bfloat16, requires_grad=True)
+    before = torch.cuda.memory_allocated()
+    torch.cuda.reset_peak_memory_stats()
+    y = linear(x, w)
+    # the padded weight and result, and the result without its padding
+    assert torch.cuda.max_memory_allocated() - before <= 2 * (1008 * 1024 + 16384 * 1008 + y.numel()) + (4 << 20)
+    w = torch.randn(1024, 9, device="cuda", dtype=torch.bfloat16)
+    r = torch.randn(16384, 1024, device="cuda", dtype=torch.bfloat16)
+    x = torch.randn(16384, 9, device="cuda", dtype=torch.bfloat16)
+    before = torch.cuda.memory_allocated()
+    torch.cuda.reset_peak_memory_stats()
+    y = linear(x, w, residual=r)
+    assert torch.cuda.max_memory_allocated() - before <= 2 * (16384 * 16 + 1024 * 16 + y.numel()) + (4 << 20)
